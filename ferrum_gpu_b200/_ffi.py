@@ -33,6 +33,7 @@ STATUS_NAMES = {
 }
 
 FC_F32, FC_Q8_0, FC_Q4_0, FC_F16, FC_FP8_E4M3, FC_FP8_E5M2, FC_MXFP4, FC_Q2_K = 0, 1, 2, 3, 4, 5, 6, 7
+FC_BF16 = 8  # an element type of the paged-cache operators, not a weight format
 FC_ROPE_NORM, FC_ROPE_NEOX = 0, 1
 FC_EXACT_F32, FC_TENSOR_F16 = 0, 1
 
@@ -105,6 +106,22 @@ class FcGpt2Tensors(C.Structure):
                 ("head", FcTensor)]
 
 
+class FcPagedCache(C.Structure):
+    _fields_ = [("page", C.c_uint32), ("n_pages", C.c_uint32), ("kv_heads", C.c_uint32), ("head_dim", C.c_uint32), ("kind", C.c_int),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("requests", C.c_uint32), ("max_pages", C.c_uint32), ("table", C.c_void_p),
+                ("lens", C.c_void_p), ("free", C.c_void_p), ("n_free", C.c_void_p)]
+
+
+class FcRotary(C.Structure):
+    _fields_ = [("cos", C.c_void_p), ("sin", C.c_void_p), ("positions", C.c_uint32), ("rope_dim", C.c_uint32), ("rope_type", C.c_uint32)]
+
+
+class FcRopeScaling(C.Structure):
+    _fields_ = [("rope_dim", C.c_uint32), ("base", C.c_float), ("linear_factor", C.c_float), ("n_freq_factors", C.c_uint32),
+                ("freq_factors", f32p), ("original_ctx", C.c_uint32), ("factor", C.c_float), ("beta_fast", C.c_float),
+                ("beta_slow", C.c_float), ("attn_factor", C.c_float)]
+
+
 # Every symbol include/ferrum_cuda.h declares; tests check that the built library exports them.
 EXPORTS = (
     "fc_device_open", "fc_device_close", "fc_device_name", "fc_device_props", "fc_last_error",
@@ -121,6 +138,7 @@ EXPORTS = (
     "fc_model_score_dev", "fc_model_set_head_shard", "fc_model_trunk_dev",
     "fc_model_head_partial_dev", "fc_score_combine_dev",
     "fc_model_score_ragged", "fc_score_windows", "fc_model_token_logprobs",
+    "fc_rope_tables", "fc_paged_extend_dev", "fc_paged_release_dev", "fc_paged_append_dev", "fc_paged_attend_dev", "fc_logprobs_dev",
     "fc_group_sequences", "fc_group_unique_id", "fc_group_create", "fc_group_destroy", "fc_group_score",
     "fc_group_last_exchange_ms",
 )
@@ -201,6 +219,12 @@ def load() -> C.CDLL:
         "fc_model_score_ragged": (C.c_int, [vp, vp, vp, u32, C.c_int, vp, vp, vp]),
         "fc_score_windows": (u32, [u32, u32, u32, vp, vp, vp, u32]),
         "fc_model_token_logprobs": (C.c_int, [vp, vp, vp, vp, u32, C.c_int, vp, vp, vp]),
+        "fc_rope_tables": (C.c_int, [P(FcRopeScaling), u32, vp, vp]),
+        "fc_paged_extend_dev": (C.c_int, [vp, P(FcPagedCache), vp, vp, u32, u32, vp, vp, vp, vp, vp, vp, vp]),
+        "fc_paged_release_dev": (C.c_int, [vp, P(FcPagedCache), vp, u32, vp, vp, vp]),
+        "fc_paged_append_dev": (C.c_int, [vp, P(FcPagedCache), P(FcRotary), vp, C.c_int, u64, u32, u32, vp, vp, vp, u64]),
+        "fc_paged_attend_dev": (C.c_int, [vp, P(FcPagedCache), vp, C.c_int, u64, u32, u32, vp, vp, C.c_float, vp, u64]),
+        "fc_logprobs_dev": (C.c_int, [vp, vp, C.c_int, u32, u64, u32, vp, u32, vp, vp, vp, vp, vp]),
         "fc_group_sequences": (u32, [u32, u32, u32, vp, u32]),
         "fc_group_unique_id": (C.c_int, [vp, sz]),
         "fc_group_create": (C.c_int, [vp, vp, u32, u32, u32, vp, sz, P(vp)]),

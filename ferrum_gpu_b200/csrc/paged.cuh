@@ -1,0 +1,31 @@
+// What the kernels of serving from a paged cache share: the three element types of activations, caches and logits, and the
+// checks of a cache's view.
+#pragma once
+#include "common.cuh"
+
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T>
+__device__ __forceinline__ T from_f32(float v);
+template <>
+__device__ __forceinline__ float from_f32<float>(float v) {
+  return v;
+}
+template <>
+__device__ __forceinline__ __half from_f32<__half>(float v) {
+  return __float2half_rn(v);
+}
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+static inline bool paged_kind(int kind) { return kind == FC_F32 || kind == FC_F16 || kind == FC_BF16; }
+static inline size_t paged_bytes(int kind) { return kind == FC_F32 ? 4 : 2; }
+static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }
+constexpr uint32_t PAGED_MAX_PAGE = 256, PAGED_MAX_HEAD_DIM = 256;
+
+// paged_plan.cu: the fields of a view that every entry point reads, and those of its k and v
+int paged_check_pages(FcDevice* dev, const FcPagedCache* c);
+int paged_check_pool(FcDevice* dev, const FcPagedCache* c);

@@ -76,6 +76,12 @@ class Device:
     def stream(self) -> int:
         return self._lib.fc_device_stream(self._h) or 0
 
+    def torch_stream(self):
+        """The handle's stream for torch: `with torch.cuda.stream(dev.torch_stream()):` puts torch's work, and the memory its
+        allocator hands out, in order with the library's calls."""
+        import torch
+        return torch.cuda.ExternalStream(self.stream(), device=f"cuda:{self.ordinal}")
+
     def launch_count(self) -> int:
         return self._lib.fc_device_launch_count(self._h)
 

@@ -1,0 +1,244 @@
+"""Serving from a paged key-value cache: the operators between the products of a step that mixes requests of unequal
+length. `PagedCache.extend` gives every new token of a step a page and a slot, `append` rotates q and k and writes k and v
+there, `attend` lets the tokens look at their requests' pages, `logprobs` answers with probabilities, and `release` gives
+the pages of finished requests back.
+
+Tensors are torch CUDA tensors that the caller owns; every call enqueues on the device handle's stream and returns. Work
+that torch does on them belongs on the same stream (`with torch.cuda.stream(dev.torch_stream()):`) or behind a
+synchronisation. Arguments are checked on the host (`CudaError`, as everywhere in this package); what only the device knows
+- lengths, free pages - is reported in `Step.status`, which the caller reads when it reads results."""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Any
+
+import numpy as np
+
+from . import _ffi
+from .device import CudaError, Device
+
+_KINDS = {"torch.float32": _ffi.FC_F32, "torch.float16": _ffi.FC_F16, "torch.bfloat16": _ffi.FC_BF16}
+
+
+def _kind(t) -> int:
+    kind = _KINDS.get(str(t.dtype))
+    if kind is None:
+        raise CudaError(_ffi.FC_ERR_UNSUPPORTED, f"elements are float32, float16 or bfloat16, not {t.dtype}")
+    return kind
+
+
+def _need(ok, code: int, message: str):
+    if not ok:
+        raise CudaError(code, message)
+
+
+def _ints(dev: Device, t, name: str, n: int | None = None, dtype: str = "torch.int32"):
+    """The address of a contiguous device tensor of whole numbers (None: NULL)."""
+    if t is None:
+        return None
+    _need(str(t.dtype) == dtype and t.is_contiguous() and t.is_cuda and t.device.index == dev.ordinal, _ffi.FC_ERR_ARG,
+          f"{name} must be a contiguous {dtype} tensor on cuda:{dev.ordinal}")
+    _need(n is None or t.numel() >= n, _ffi.FC_ERR_SHAPE, f"{name} has {t.numel()} entries, needs {n}")
+    return t.data_ptr()
+
+
+def _rows(dev: Device, t, name: str):
+    """(address, kind, stride) of a two-dimensional device tensor whose rows are contiguous."""
+    _need(t.dim() == 2 and t.is_cuda and t.device.index == dev.ordinal, _ffi.FC_ERR_ARG, f"{name} must be rows on cuda:{dev.ordinal}")
+    _need(t.shape[1] <= 1 or t.stride(1) == 1, _ffi.FC_ERR_ARG, f"the elements of {name}'s rows must lie side by side")
+    return t.data_ptr(), _kind(t), max(0, t.stride(0))
+
+
+@dataclass
+class RopeScaling:
+    """How rotary angles are scaled (FcRopeScaling): `linear_factor` and `freq_factors` as in the Llama configuration;
+    `original_ctx` != 0 stretches the context by `factor` the YaRN way. `attn_factor` 0: 0.1 ln(factor) + 1."""
+    rope_dim: int
+    base: float = 10000.0
+    linear_factor: float = 1.0
+    freq_factors: np.ndarray | None = None
+    original_ctx: int = 0
+    factor: float = 1.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attn_factor: float = 0.0
+
+
+def rope_tables(scaling: RopeScaling, positions: int):
+    """cos and sin [positions, rope_dim / 2], f32 numpy arrays; host arithmetic in 64 bits."""
+    s, lib = scaling, _ffi.load()
+    ff = None if s.freq_factors is None else np.ascontiguousarray(s.freq_factors, dtype=np.float32)
+    c = _ffi.FcRopeScaling(s.rope_dim, s.base, s.linear_factor, 0 if ff is None else ff.size,
+                           None if ff is None else ff.ctypes.data_as(_ffi.f32p), s.original_ctx, s.factor, s.beta_fast, s.beta_slow,
+                           s.attn_factor)
+    cos, sin = (np.empty((positions, max(0, s.rope_dim) // 2), dtype=np.float32) for _ in range(2))
+    rc = lib.fc_rope_tables(C.byref(c), positions, cos.ctypes.data, sin.ctypes.data)
+    if rc != _ffi.FC_OK:
+        raise CudaError(rc, lib.fc_last_error(None).decode())
+    return cos, sin
+
+
+class Rotary:
+    """Rotary tables on the device: f32 [positions, rope_dim / 2] each; `neox` pairs channel p with p + rope_dim / 2, else
+    neighbours are pairs. Channels from rope_dim on stay as they are."""
+
+    def __init__(self, cos, sin, neox: bool):
+        for t, name in ((cos, "cos"), (sin, "sin")):
+            _need(t.dim() == 2 and str(t.dtype) == "torch.float32" and t.is_contiguous() and t.is_cuda and t.shape == cos.shape, _ffi.FC_ERR_ARG,
+                  f"{name} must be a contiguous float32 [positions, rope_dim / 2] tensor on the device")
+        self.cos, self.sin = cos, sin
+        self._c = _ffi.FcRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+                                _ffi.FC_ROPE_NEOX if neox else _ffi.FC_ROPE_NORM)
+
+    @classmethod
+    def build(cls, dev: Device, scaling: RopeScaling, positions: int, neox: bool) -> "Rotary":
+        import torch
+        cos, sin = (torch.from_numpy(t).to(f"cuda:{dev.ordinal}") for t in rope_tables(scaling, positions))
+        torch.cuda.synchronize(dev.ordinal)
+        return cls(cos, sin, neox)
+
+
+@dataclass
+class Step:
+    """The rows of one step. `extend` fills all of it; `append` reads slot and position, `attend` position and request.
+    Rows past the step's tokens have -1 everywhere."""
+    starts: Any = None    # int32 [requests of the step + 1]: each one's first row, and the total
+    slot: Any = None      # int64 [rows]
+    position: Any = None  # int32 [rows]
+    request: Any = None   # int32 [rows]: the row of the page table
+    status: Any = None    # int32 [1]: 0, the number of pages that are missing, or an FC_ERR_* code
+
+    @classmethod
+    def new(cls, dev: Device, requests: int, rows: int) -> "Step":
+        import torch
+        with torch.cuda.stream(dev.torch_stream()):
+            def ints(n, dtype=torch.int32):
+                return torch.full((n,), -1, dtype=dtype, device=f"cuda:{dev.ordinal}")
+            return cls(ints(requests + 1), ints(rows, torch.int64), ints(rows), ints(rows), ints(1))
+
+
+class PagedCache:
+    """A paged key-value cache over the caller's tensors: `layers` pairs (k, v) of [pages, kv_heads, page, head_dim], the page
+    `table` int32 [requests, max_pages], `lens` int32 [requests], and the stack of `free` pages int32 [pages] with its height
+    `n_free` int32 [1]. What a call does not use may be left out."""
+
+    def __init__(self, dev: Device, page: int, table=None, lens=None, free=None, n_free=None, layers=()):
+        self.dev, self._lib, self.page = dev, _ffi.load(), page
+        self.table, self.lens, self.free, self.n_free, self.layers = table, lens, free, n_free, list(layers)
+        shapes = {(tuple(t.shape), str(t.dtype)) for kv in self.layers for t in kv}
+        _need(len(shapes) <= 1, _ffi.FC_ERR_SHAPE, "every layer's k and v must have one shape and type")
+        for kv in self.layers:
+            for t in kv:
+                _need(t.dim() == 4 and t.shape[2] == page and t.is_contiguous() and t.is_cuda and t.device.index == dev.ordinal,
+                      _ffi.FC_ERR_ARG, f"k and v must be contiguous [pages, kv_heads, {page}, head_dim] tensors on cuda:{dev.ordinal}")
+        _need(table is None or table.dim() == 2, _ffi.FC_ERR_SHAPE, "the page table must be [requests, max_pages]")
+        requests, most = (0, 0) if table is None else table.shape
+        pages = self.layers[0][0].shape[0] if self.layers else free.numel() if free is not None else 0
+        _need(free is None or free.numel() == pages, _ffi.FC_ERR_SHAPE, "the stack of free pages has another length than the pool")
+        self._plan = (_ints(dev, table, "table"), _ints(dev, lens, "lens", requests), _ints(dev, free, "free"), _ints(dev, n_free, "n_free", 1))
+        self._views = []
+        for k, v in self.layers or [(None, None)]:
+            kv_heads, head_dim, kind = (0, 0, 0) if k is None else (k.shape[1], k.shape[3], _kind(k))
+            self._views.append(_ffi.FcPagedCache(page, pages, kv_heads, head_dim, kind, None if k is None else k.data_ptr(),
+                                                 None if v is None else v.data_ptr(), requests, most, *self._plan))
+
+    @classmethod
+    def new(cls, dev: Device, layers: int, kv_heads: int, head_dim: int, pages: int, page: int, requests: int, max_pages: int,
+            dtype) -> "PagedCache":
+        """An empty cache: every page free, the first page on top of the stack."""
+        import torch
+        where = f"cuda:{dev.ordinal}"
+        with torch.cuda.stream(dev.torch_stream()):
+            kv = [tuple(torch.empty(pages, kv_heads, page, head_dim, dtype=dtype, device=where) for _ in range(2)) for _ in range(layers)]
+            return cls(dev, page, torch.full((requests, max_pages), -1, dtype=torch.int32, device=where),
+                       torch.zeros(requests, dtype=torch.int32, device=where),
+                       torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=where),
+                       torch.full((1,), pages, dtype=torch.int32, device=where), kv)
+
+    def extend(self, grow, step: Step, requests=None, lens_out=None, n_free_out=None):
+        """Pages, slots and positions of the step's tokens: request `requests[i]` (a row of the table; None: i) grows by
+        `grow[i]` tokens. All or nothing: see `Step.status`. Lengths and stack height change in place unless others are given."""
+        dev, n = self.dev, grow.numel()
+        rows = {t.numel() for t in (step.slot, step.position, step.request) if t is not None}
+        _need(len(rows) <= 1, _ffi.FC_ERR_SHAPE, "slot, position and request of a step must have one length")
+        dev.check(self._lib.fc_paged_extend_dev(
+            dev.handle, C.byref(self._views[0]), _ints(dev, requests, "requests", n), _ints(dev, grow, "grow"), n, rows.pop() if rows else 0,
+            _ints(dev, step.starts, "starts", n + 1), _ints(dev, step.slot, "slot", dtype="torch.int64"), _ints(dev, step.position, "position"),
+            _ints(dev, step.request, "request"), self._lens_out(lens_out), _ints(dev, n_free_out, "n_free_out", 1),
+            _ints(dev, step.status, "status", 1)))
+
+    def release(self, requests, status, lens_out=None, n_free_out=None):
+        """All pages of these requests back onto the stack, their lengths 0."""
+        dev = self.dev
+        dev.check(self._lib.fc_paged_release_dev(dev.handle, C.byref(self._views[0]), _ints(dev, requests, "requests"), requests.numel(),
+                                                 self._lens_out(lens_out), _ints(dev, n_free_out, "n_free_out", 1),
+                                                 _ints(dev, status, "status", 1)))
+
+    def _lens_out(self, t):
+        return _ints(self.dev, t, "lens_out", 0 if self.table is None else self.table.shape[0])
+
+    def append(self, layer: int, qkv, step: Step, q_out, rotary: Rotary | None = None):
+        """Rows q heads | k heads | v heads: q and k rotated by `rotary` (None: not), q to the rows of `q_out`, k and v to the
+        cache's slots. `q_out` may be the q part of `qkv`."""
+        dev, view = self.dev, self._view(layer)
+        at, kind, stride = _rows(dev, qkv, "qkv")
+        q_at, q_kind, q_stride = _rows(dev, q_out, "q_out")
+        rows, width = qkv.shape
+        hd, kv = view.head_dim, view.kv_heads
+        heads = width // hd - 2 * kv
+        _need(width % hd == 0 and heads > 0, _ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {hd} beside {2 * kv}")
+        _need(q_kind == kind and tuple(q_out.shape) == (rows, heads * hd), _ffi.FC_ERR_SHAPE, f"q_out must be {rows} x {heads * hd} of qkv's type")
+        dev.check(self._lib.fc_paged_append_dev(dev.handle, C.byref(view), C.byref(rotary._c) if rotary is not None else None, at, kind, stride,
+                                                rows, heads, _ints(dev, step.slot, "slot", rows, "torch.int64"),
+                                                _ints(dev, step.position, "position", rows), q_at, q_stride))
+
+    def attend(self, layer: int, q, step: Step, out, scale: float = 0.0):
+        """Every row of `q` over positions 0 .. position of its request; `scale` 0 is 1 / sqrt(head_dim)."""
+        dev, view = self.dev, self._view(layer)
+        at, kind, stride = _rows(dev, q, "q")
+        out_at, out_kind, out_stride = _rows(dev, out, "out")
+        rows, width = q.shape
+        _need(width % view.head_dim == 0, _ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {view.head_dim}")
+        _need(out_kind == kind and out.shape == q.shape, _ffi.FC_ERR_SHAPE, "the result must have q's shape and type")
+        dev.check(self._lib.fc_paged_attend_dev(dev.handle, C.byref(view), at, kind, stride, rows, width // view.head_dim,
+                                                _ints(dev, step.request, "request", rows), _ints(dev, step.position, "position", rows),
+                                                float(scale), out_at, out_stride))
+
+    def _view(self, layer: int):
+        _need(self.layers and 0 <= layer < len(self.layers), _ffi.FC_ERR_RANGE, f"layer {layer} of {len(self.layers)}")
+        return self._views[layer]
+
+
+@dataclass
+class LogProbs:
+    """Where `logprobs` puts its results; what is None is not computed."""
+    logprob: Any = None      # f32 [rows]: of the target; NaN where there is none
+    entropy: Any = None      # f32 [rows], nats
+    rank: Any = None         # int32 [rows]: 0 is the greedy pick; -1 where there is no target
+    top_index: Any = None    # int32 [rows, top]
+    top_logprob: Any = None  # f32 [rows, top]
+
+    @classmethod
+    def new(cls, dev: Device, rows: int, top: int) -> "LogProbs":
+        import torch
+        where = f"cuda:{dev.ordinal}"
+        with torch.cuda.stream(dev.torch_stream()):
+            f, i = (dict(dtype=t, device=where) for t in (torch.float32, torch.int32))
+            return cls(torch.empty(rows, **f), torch.empty(rows, **f), torch.empty(rows, **i), torch.empty(rows, top, **i),
+                       torch.empty(rows, top, **f))
+
+
+def logprobs(dev: Device, logits, targets, out: LogProbs, vocab: int | None = None):
+    """Log-probability and rank of `targets` (int32 [rows], -1: none; None: nowhere), entropy and the largest alternatives of
+    the first `vocab` elements (None: all) of every row of `logits`."""
+    lib = _ffi.load()
+    at, kind, stride = _rows(dev, logits, "logits")
+    rows, width = logits.shape
+    _need(vocab is None or 0 < vocab <= width, _ffi.FC_ERR_SHAPE, f"{vocab} logits of rows of {width}")
+    tops = {tuple(t.shape) for t in (out.top_index, out.top_logprob) if t is not None}
+    _need(len(tops) <= 1 and all(len(s) == 2 and s[0] == rows for s in tops), _ffi.FC_ERR_SHAPE, f"the alternatives must be {rows} rows of one width")
+    dev.check(lib.fc_logprobs_dev(dev.handle, at, kind, rows, stride, width if vocab is None else vocab, _ints(dev, targets, "targets", rows),
+                                  tops.pop()[1] if tops else 0, _ints(dev, out.logprob, "logprob", rows, "torch.float32"),
+                                  _ints(dev, out.entropy, "entropy", rows, "torch.float32"), _ints(dev, out.rank, "rank", rows),
+                                  _ints(dev, out.top_index, "top_index"), _ints(dev, out.top_logprob, "top_logprob", dtype="torch.float32")))

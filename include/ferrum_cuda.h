@@ -422,6 +422,115 @@ int fc_model_token_logprobs(FcModel* m, const int32_t* ids, const uint32_t* offs
                             uint32_t n_streams, int mode, double* logprob_out, uint64_t* n_tokens_out,
                             uint8_t* greedy_out);
 
+/* ---- serving from a paged key-value cache --------------------------------------------------------
+ * What a server needs between requests of unequal length and a fixed memory, and the resident models' caches (one
+ * [stream][kv_head][ctx][head_dim] reserve per stream) do not give: positions of all requests live in pages of one pool,
+ * page tables say which. None of these entry points has a counterpart in the reference, whose cache is per model.
+ * One serving step: fc_paged_extend_dev (pages and slots of the step's new tokens), per layer fc_paged_append_dev (q and k
+ * rotated, k and v written to their slots) and fc_paged_attend_dev (the tokens over their requests' pages), then
+ * fc_logprobs_dev on the logits; fc_paged_release_dev when requests end. All memory is the caller's, on the device, and
+ * everything is enqueued on the handle's stream without synchronising; what a call leaves in one buffer the next may read.
+ * A step's rows may be more than its tokens (a fixed shape for a captured graph): the rows left over have position -1. */
+
+/* Plain bf16 values in the buffers of this section (not a weight format). The element types here are FC_F32, FC_F16 and
+ * FC_BF16; sums, softmax statistics and log-probabilities are f32 whatever they are. */
+enum { FC_BF16 = 8 };
+
+/* A view of a paged cache: pointers and sizes, nothing that the library keeps. An entry point reads the fields it names;
+ * the others may be zero. One view per layer: k and v differ, the rest is shared. */
+typedef struct {
+  uint32_t page;      /* positions per page: a power of two, 1..256 */
+  uint32_t n_pages;   /* pages of the pool */
+  uint32_t kv_heads;
+  uint32_t head_dim;  /* a multiple of 8, 8..256 */
+  int kind;           /* element type of k and v */
+  void *k, *v;        /* [n_pages][kv_heads][page][head_dim], 16-byte aligned */
+  uint32_t requests;  /* rows of the table */
+  uint32_t max_pages; /* columns of the table */
+  int32_t* table;     /* [requests][max_pages]: the page that holds positions [i * page, (i + 1) * page) of a request */
+  int32_t* lens;      /* [requests]: positions held */
+  int32_t* free;      /* [n_pages]: a stack of the pages nobody holds ... */
+  int32_t* n_free;    /* [1]: ... and its height */
+} FcPagedCache;
+
+/* Rotary tables on the device: cos and sin [positions][rope_dim / 2]; rope_type FC_ROPE_NORM pairs channels (2p, 2p + 1),
+ * FC_ROPE_NEOX (p, p + rope_dim / 2); channels from rope_dim on are left as they are. */
+typedef struct {
+  const float *cos, *sin;
+  uint32_t positions, rope_dim, rope_type;
+} FcRotary;
+
+/* How the angles of fc_rope_tables are scaled: freq_i = base^(-2i / rope_dim), divided by linear_factor and by
+ * freq_factors[i] as in FcLlamaConfig; with original_ctx != 0 also stretched by `factor` the YaRN way (Peng et al. 2023):
+ * pairs that turn less than beta_slow times in original_ctx positions are slowed by `factor`, those that turn more than
+ * beta_fast times are kept, the ones between mix along the pair's index, and cos and sin are multiplied by attn_factor
+ * (0: 0.1 ln(factor) + 1). */
+typedef struct {
+  uint32_t rope_dim;
+  float base, linear_factor;
+  uint32_t n_freq_factors; /* 0 or rope_dim / 2 */
+  const float* freq_factors;
+  uint32_t original_ctx; /* 0: no stretching */
+  float factor, beta_fast, beta_slow, attn_factor;
+} FcRopeScaling;
+/* Fills host arrays [positions][rope_dim / 2]. Angles are formed in 64 bits and rounded once, as cos and sin. Host
+ * arithmetic, no device. */
+int fc_rope_tables(const FcRopeScaling* scaling, uint32_t positions, float* cos_out, float* sin_out);
+
+/* The step's pages and slots, from the requests' lengths. Reads page, n_pages, requests, max_pages, table, lens, free,
+ * n_free. Request i of `n` (<= 8192) is table row requests_dev[i] (NULL: i; no row twice) and grows by grow_dev[i] >= 0
+ * tokens. Writes, in the order of the requests: starts_dev[n + 1] (each request's first row, and the total); for rows
+ * 0 .. rows - 1 slot_dev (page * page size + offset), position_dev and request_dev (the table row), -1 in the rows past
+ * the total; the table entries of pages newly taken from the top of the stack, lowest position first; the requests' new
+ * lengths to lens_out_dev (NULL: in place) and the stack's new height to n_free_out_dev (NULL: in place).
+ * status_dev[0]: 0; > 0: so many pages are missing; FC_ERR_RANGE: a row outside the table or a negative growth;
+ * FC_ERR_CONTEXT_FULL: a request outgrows its table row; FC_ERR_SHAPE: more tokens than rows. Unless 0, nothing is taken:
+ * no row has a token, lengths, table and stack stay. slot, position and request may each be NULL. */
+int fc_paged_extend_dev(FcDevice* dev, const FcPagedCache* cache, const int32_t* requests_dev, const int32_t* grow_dev, uint32_t n,
+                        uint32_t rows, int32_t* starts_dev, int64_t* slot_dev, int32_t* position_dev, int32_t* request_dev,
+                        int32_t* lens_out_dev, int32_t* n_free_out_dev, int32_t* status_dev);
+/* Gives back all pages of `n` requests, in order: pushed on the stack lowest position first, lengths become 0 (written
+ * like the outputs of fc_paged_extend_dev; the table's entries stay, nobody reads them past a length). status_dev[0]: 0;
+ * FC_ERR_RANGE: a row outside the table, or a length or page that is none; FC_ERR_SHAPE: the stack would grow past n_pages
+ * (a page given back twice). Unless 0, nothing changes. */
+int fc_paged_release_dev(FcDevice* dev, const FcPagedCache* cache, const int32_t* requests_dev, uint32_t n, int32_t* lens_out_dev,
+                         int32_t* n_free_out_dev, int32_t* status_dev);
+
+/* Rotates q and k and writes k and v to the cache. Reads page, n_pages, kv_heads, head_dim, kind, k, v. `qkv_dev` has
+ * `rows` rows of (heads + 2 * kv_heads) * head_dim elements of type `kind`, `stride` elements apart: q heads | k heads |
+ * v heads, what the fused product of a resident model leaves. Row r's rotated q goes to q_out_dev (type `kind`, rows
+ * q_stride elements apart; it may be the q of qkv_dev itself), its k and v to slot_dev[r], its angles are those of
+ * position_dev[r]. `rotary` NULL: nothing is rotated. A row whose slot lies outside the pool leaves the cache alone (-1 on
+ * purpose); one whose position is negative or outside the tables gives q = 0 and leaves the cache alone. No two rows may
+ * share a slot. */
+int fc_paged_append_dev(FcDevice* dev, const FcPagedCache* cache, const FcRotary* rotary, const void* qkv_dev, int kind, uint64_t stride,
+                        uint32_t rows, uint32_t heads, const int64_t* slot_dev, const int32_t* position_dev, void* q_out_dev,
+                        uint64_t q_stride);
+
+/* Attention of new tokens over the cache. Reads page, n_pages, kv_heads, head_dim, kind, k, v, requests, max_pages, table.
+ * Row r of q_dev (`rows` rows of heads * head_dim elements of type `kind`, q_stride elements apart; heads a multiple of
+ * kv_heads, consecutive heads share a kv head) attends positions 0 .. position_dev[r] of table row request_dev[r] (NULL:
+ * r); several rows may be of one request (a prompt's rows, each behind its own position). `scale` 0: 1 / sqrt(head_dim).
+ * out_dev: the same shape and type, out_stride apart, not overlapping q. A row with a negative position or a request
+ * outside the table attends nothing and gives 0; positions whose table entry is no page of the pool are left out.
+ * Scratch (a fixed few MB) belongs to the device handle and is allocated by the first call, under a stream capture too;
+ * replays of graphs that hold this call must not overlap with one another or with other work on the handle. */
+int fc_paged_attend_dev(FcDevice* dev, const FcPagedCache* cache, const void* q_dev, int kind, uint64_t q_stride, uint32_t rows,
+                        uint32_t heads, const int32_t* request_dev, const int32_t* position_dev, float scale, void* out_dev,
+                        uint64_t out_stride);
+
+/* Log-probabilities of given tokens with what a completion's answer lists beside them. `logits_dev`: `rows` rows of
+ * `vocab` elements of type `kind`, `stride` elements apart. Per row (each output may be NULL): logprob = x[target] - lse,
+ * entropy = -sum p log p in nats, rank = logits above the target's, or equal at a lower index (0: the greedy pick), and the
+ * `top` (0..32) largest logits, ties lower index first, as top_index and top_logprob [rows][top]. A target outside
+ * 0 .. vocab - 1 (or targets_dev NULL) gives logprob NaN and rank -1. Logits of -inf are forbidden tokens: probability 0,
+ * listed last; a row of nothing else has log-probabilities -inf and entropy 0. A NaN or +inf logit makes the row's
+ * log-probabilities and entropy NaN; NaN is never listed or counted, a NaN target ranks behind all others. Entries past
+ * the logits that can be listed have index -1 and log-probability -inf. -0 equals +0. */
+int fc_logprobs_dev(FcDevice* dev, const void* logits_dev, int kind, uint32_t rows, uint64_t stride, uint32_t vocab,
+                    const int32_t* targets_dev, uint32_t top, float* logprob_dev, float* entropy_dev, int32_t* rank_dev,
+                    int32_t* top_index_dev, float* top_logprob_dev);
+
 /* ---- groups of GPUs (multi-GPU scoring behind the ABI) ----------------------------------------
  * A group is `world` ranks, each with its own open device and resident model, in one or several processes
  * (one thread per rank inside a process). It owns its NCCL communicators; NCCL is loaded at run time
