@@ -39,6 +39,8 @@ struct FcDevice {
   Workspace scratch;
   uint32_t weights = 0; // stand-alone weights alive
   cudaMemPool_t workspaces = nullptr;
+  Workspace attend;          // of the attention over a paged cache, from its first call on (paged_attend.cu)
+  bool attend_clear = false; // its counters have been zeroed
   int* d_flag = nullptr;   // device int for kernels that report a status
   int matvec_choice = 0;   // fc_debug_matvec_kernel: which kernel multiplies 1..8 rows (0: the library's rule)
   // per-kernel timing (off by default): one event pair per launch, summed by name on report
