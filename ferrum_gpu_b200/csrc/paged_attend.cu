@@ -130,41 +130,42 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
   auto& sm_o = sm.o;
   __shared__ float sm_m[WARPS][ROWS8], sm_l[WARPS][ROWS8];
   __shared__ uint32_t sm_big[ROWS8];
-  __shared__ unsigned long long sm_scan[WARPS];
-  __shared__ uint32_t sm_row, sm_last;
-  __shared__ unsigned long long sm_at;
+  __shared__ uint32_t sm_scan[WARPS], sm_row, sm_at, sm_last;
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const uint32_t per_row = a.kv_heads * a.blocks;
   grid_wait();
 
   // Where this CTA's share of the tiles begins: prefix sums over the rows' tiles, a run of rows per thread.
   const uint32_t run = (a.rows + WARPS * 32 - 1) / (WARPS * 32), r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
-  unsigned long long mine = 0;
-  uint32_t req;
+  uint32_t mine = 0, req;
   for (uint32_t r = r0; r < r1; r++) mine += row_tiles(row_len(a, r, req));
-  unsigned long long upto = mine;
+  uint32_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const unsigned long long x = __shfl_up_sync(0xffffffffu, upto, o);
+    const uint32_t x = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += x;
   }
   if (lane == 31) sm_scan[warp] = upto;
   __syncthreads();
-  unsigned long long all = 0;
+  uint32_t all = 0;
 #pragma unroll
   for (int w = 0; w < WARPS; w++) {
     if (w < (int)warp) upto += sm_scan[w];
     all += sm_scan[w];
   }
   all *= per_row, upto *= per_row, mine *= per_row;
-  const unsigned long long n_cta = min((unsigned long long)gridDim.x, all);
+  const uint32_t n_cta = min(gridDim.x, all), share = all / n_cta, extra = all % n_cta; // (the first `extra` CTAs take one more)
   if (blockIdx.x >= n_cta) return;
-  const unsigned long long begin = blockIdx.x * all / n_cta, end = (blockIdx.x + 1) * all / n_cta;
+  auto begin_of = [&](uint32_t c) { return c * share + min(c, extra); };
+  auto owner_of = [&](uint32_t tile) {
+    const uint32_t longer = extra * (share + 1);
+    return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+  };
+  const uint32_t begin = begin_of(blockIdx.x), end = begin_of(blockIdx.x + 1);
   if (upto - mine <= begin && begin < upto) {
-    unsigned long long at = upto - mine;
-    uint32_t r = r0;
+    uint32_t at = upto - mine, r = r0;
     for (;; r++) {
-      const unsigned long long n = (unsigned long long)row_tiles(row_len(a, r, req)) * per_row;
+      const uint32_t n = row_tiles(row_len(a, r, req)) * per_row;
       if (begin < at + n) break;
       at += n;
     }
@@ -172,12 +173,12 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
   }
   __syncthreads();
   uint32_t r = sm_row, len = row_len(a, r, req), tiles = row_tiles(len);
-  unsigned long long row_at = sm_at; // the row's first tile
-  uint32_t which = (uint32_t)((begin - row_at) / tiles), tile = (uint32_t)((begin - row_at) % tiles);
+  uint32_t row_at = sm_at; // the row's first tile
+  uint32_t which = (begin - row_at) / tiles, tile = (begin - row_at) % tiles;
 
   const size_t row_bytes = (size_t)a.hd * sizeof(C);
-  for (unsigned long long at = begin; at < end;) {
-    const uint32_t tile_end = (uint32_t)min((unsigned long long)tiles, tile + (end - at));
+  for (uint32_t at = begin; at < end;) {
+    const uint32_t tile_end = min(tiles, tile + (end - at));
     const uint32_t kvh = which / a.blocks, h0 = kvh * a.group + (which % a.blocks) * ROWS8;
     const uint32_t heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
     // q's terms as the matrix operand wants them: lane (g, t) of piece j has channels (4 j + t) E .. of head h0 + g
@@ -404,11 +405,10 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
         for (int x = 0; x < 2; x++) sm_o[warp][g][(8 * i + 2 * t + x) * E + e] = o[i][e][x] + o[i][e][x + 2];
     __syncthreads();
     const bool whole = tile == 0 && tile_end == tiles;
-    const unsigned long long first_tile = row_at + (unsigned long long)which * tiles, last_tile = first_tile + tiles - 1;
-    // (CTA c begins at tile c all / n_cta: the owner of a tile)
-    const uint32_t c0 = whole ? 0 : (uint32_t)(((first_tile + 1) * n_cta - 1) / all), c1 = whole ? 0 : (uint32_t)(((last_tile + 1) * n_cta - 1) / all);
+    const uint32_t first_tile = row_at + which * tiles;
+    const uint32_t c0 = whole ? 0 : owner_of(first_tile), c1 = whole ? 0 : owner_of(first_tile + tiles - 1);
     auto part_of = [&](uint32_t c) { // a CTA has two: one for where it begins, one for where it ends
-      return a.parts + (size_t)(2 * c + (c * all / n_cta >= first_tile ? 0 : 1)) * part_floats(HDP);
+      return a.parts + (size_t)(2 * c + (begin_of(c) >= first_tile ? 0 : 1)) * part_floats(HDP);
     };
     float* part = whole ? nullptr : part_of(blockIdx.x);
     for (uint32_t i = tid; i < heads * a.hd; i += WARPS * 32) {
@@ -437,18 +437,55 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
       __syncthreads();
       if (sm_last) {
         __threadfence();
-        for (uint32_t i = tid; i < heads * a.hd; i += WARPS * 32) {
-          const uint32_t h = i / a.hd, ch = i - h * a.hd;
+        // Each warp finds two heads' maxima over the parts; then, JOIN parts at a time, their weights go to shared memory and
+        // every thread adds its channels' values, all loads of a turn in flight together.
+        float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(&sm);
+        constexpr int JOIN = 32, OWN = (ROWS8 * HDP / 4 + WARPS * 32 - 1) / (WARPS * 32);
+        {
+          const uint32_t h = warp * 2 + (lane >> 4);
           float m = -INFINITY;
-          for (uint32_t c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(part_of(c) + h));
-          const float base = m == -INFINITY ? 0.0f : m;
-          float l = 0.0f, v = 0.0f;
-          for (uint32_t c = c0; c <= c1; c++) {
-            const float* q = part_of(c);
-            const float f = ex2(__ldcg(q + h) - base);
-            l = fmaf(__ldcg(q + ROWS8 + h), f, l), v = fmaf(__ldcg(q + 2 * ROWS8 + h * HDP + ch), f, v);
+          for (uint32_t c = c0 + (lane & 15); c <= c1; c += 16) m = fmaxf(m, __ldcg(part_of(c) + h));
+#pragma unroll
+          for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          sm_m[0][h] = m == -INFINITY ? 0.0f : m; // (all lanes of a head write the same)
+        }
+        __syncthreads();
+        float4 v[OWN];
+        float l[OWN];
+#pragma unroll
+        for (int n = 0; n < OWN; n++) v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l[n] = 0.0f;
+        for (uint32_t c = c0; c <= c1; c += JOIN) {
+          const uint32_t here = min((uint32_t)JOIN, c1 - c + 1);
+          for (uint32_t i = tid; i < here * ROWS8; i += WARPS * 32) {
+            const uint32_t h = i % ROWS8;
+            const float* q = part_of(c + i / ROWS8);
+            const float f = ex2(__ldcg(q + h) - sm_m[0][h]);
+            sm_w[i / ROWS8][h] = f, sm_w[JOIN + i / ROWS8][h] = f * __ldcg(q + ROWS8 + h);
           }
-          store_act(a.out, a.act, (size_t)r * a.out_stride + (size_t)(h0 + h) * a.hd + ch, l == 0.0f ? 0.0f : v / l);
+          __syncthreads();
+#pragma unroll
+          for (int n = 0; n < OWN; n++) {
+            const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
+            if (h >= heads || (!FULL && ch >= a.hd)) continue;
+            const float* q = a.parts + 2 * ROWS8 + h * HDP + ch;
+#pragma unroll 8
+            for (uint32_t k = 0; k < here; k++) {
+              const float4 x = __ldcg(reinterpret_cast<const float4*>(q + (part_of(c + k) - a.parts)));
+              const float f = sm_w[k][h];
+              v[n].x = fmaf(x.x, f, v[n].x), v[n].y = fmaf(x.y, f, v[n].y), v[n].z = fmaf(x.z, f, v[n].z), v[n].w = fmaf(x.w, f, v[n].w);
+              l[n] += sm_w[JOIN + k][h];
+            }
+          }
+          __syncthreads();
+        }
+#pragma unroll
+        for (int n = 0; n < OWN; n++) {
+          const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
+          if (h >= heads || (!FULL && ch >= a.hd)) continue;
+          const float f = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
+          const float x[4] = {v[n].x * f, v[n].y * f, v[n].z * f, v[n].w * f};
+#pragma unroll
+          for (int e = 0; e < 4; e++) store_act(a.out, a.act, (size_t)r * a.out_stride + (size_t)(h0 + h) * a.hd + ch + e, x[e]);
         }
         if (tid == 0) a.arrived[c0] = 0; // for the next call
       }
@@ -457,7 +494,7 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
     at += tile_end - tile;
     tile = 0;
     if (tile_end == tiles && ++which == per_row) {
-      row_at += (unsigned long long)tiles * per_row;
+      row_at += tiles * per_row;
       which = 0;
       if (++r < a.rows) len = row_len(a, r, req), tiles = row_tiles(len);
     }
@@ -535,6 +572,10 @@ FC_API int fc_paged_attend_dev(FcDevice* dev, const FcPagedCache* c, const void*
   if (!std::isfinite(scale)) return fc_fail(dev, FC_ERR_ARG, "the scale is not finite");
   if (!request && rows > c->requests) return fc_fail(dev, FC_ERR_RANGE, "%u rows in a table of %u requests", rows, c->requests);
   if (!rows) return FC_OK;
+  const uint64_t row_most = ((uint64_t)c->max_pages * c->page + TILE - 1) / TILE;
+  if ((uint64_t)rows * heads * row_most > 0xffffffffull) // (tiles are counted in 32 bits)
+    return fc_fail(dev, FC_ERR_UNSUPPORTED, "%u rows of %u heads over page tables of %u x %u positions: more than one call holds", rows, heads,
+                   c->max_pages, c->page);
   AttendArgs a = {};
   a.q = q, a.k = c->k, a.v = c->v, a.out = out, a.request = request, a.position = position, a.table = c->table;
   a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.kv_heads = c->kv_heads, a.hd = c->head_dim;

@@ -10,7 +10,7 @@ synchronisation. Arguments are checked on the host (`CudaError`, as everywhere i
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
+from dataclasses import dataclass, fields
 from typing import Any
 
 import numpy as np
@@ -18,11 +18,14 @@ import numpy as np
 from . import _ffi
 from .device import CudaError, Device
 
-_KINDS = {"torch.float32": _ffi.FC_F32, "torch.float16": _ffi.FC_F16, "torch.bfloat16": _ffi.FC_BF16}
+_KINDS: dict = {}  # torch's element types -> FC_*, filled when the first tensor comes by: the package loads without torch
 
 
 def _kind(t) -> int:
-    kind = _KINDS.get(str(t.dtype))
+    if not _KINDS:
+        import torch
+        _KINDS.update({torch.float32: _ffi.FC_F32, torch.float16: _ffi.FC_F16, torch.bfloat16: _ffi.FC_BF16})
+    kind = _KINDS.get(t.dtype)
     if kind is None:
         raise CudaError(_ffi.FC_ERR_UNSUPPORTED, f"elements are float32, float16 or bfloat16, not {t.dtype}")
     return kind
@@ -33,21 +36,52 @@ def _need(ok, code: int, message: str):
         raise CudaError(code, message)
 
 
-def _ints(dev: Device, t, name: str, n: int | None = None, dtype: str = "torch.int32"):
-    """The address of a contiguous device tensor of whole numbers (None: NULL)."""
+def _flat(t, name: str, dtype: str = "torch.int32"):
+    """(address, entries, device) of a contiguous device tensor, all of it; None: nothing."""
     if t is None:
-        return None
-    _need(str(t.dtype) == dtype and t.is_contiguous() and t.is_cuda and t.device.index == dev.ordinal, _ffi.FC_ERR_ARG,
-          f"{name} must be a contiguous {dtype} tensor on cuda:{dev.ordinal}")
-    _need(n is None or t.numel() >= n, _ffi.FC_ERR_SHAPE, f"{name} has {t.numel()} entries, needs {n}")
-    return t.data_ptr()
+        return None, None, None
+    if not (t.is_cuda and t.is_contiguous() and str(t.dtype) == dtype):
+        raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be a contiguous {dtype} tensor on the device")
+    return t.data_ptr(), t.numel(), t.get_device()
+
+
+def _ints(dev: Device, t, name: str, n: int = 0):
+    """The address of a contiguous int32 tensor of at least `n` entries on `dev`; None: NULL."""
+    at, entries, where = _flat(t, name)
+    if at is not None:
+        _at(dev, name, n, entries, where)
+    return at
+
+
+def _at(dev: Device, name: str, n: int, entries: int, where: int):
+    if where != dev.ordinal:
+        raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be on cuda:{dev.ordinal}")
+    if entries < n:
+        raise CudaError(_ffi.FC_ERR_SHAPE, f"{name} has {entries} entries, needs {n}")
 
 
 def _rows(dev: Device, t, name: str):
     """(address, kind, stride) of a two-dimensional device tensor whose rows are contiguous."""
-    _need(t.dim() == 2 and t.is_cuda and t.device.index == dev.ordinal, _ffi.FC_ERR_ARG, f"{name} must be rows on cuda:{dev.ordinal}")
-    _need(t.shape[1] <= 1 or t.stride(1) == 1, _ffi.FC_ERR_ARG, f"the elements of {name}'s rows must lie side by side")
-    return t.data_ptr(), _kind(t), max(0, t.stride(0))
+    if t.dim() != 2 or t.get_device() != dev.ordinal or not t.is_cuda:
+        raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be rows on cuda:{dev.ordinal}")
+    stride, step = t.stride()
+    if step != 1 and t.shape[1] > 1:
+        raise CudaError(_ffi.FC_ERR_ARG, f"the elements of {name}'s rows must lie side by side")
+    return t.data_ptr(), _kind(t), stride
+
+
+class _Buffers:
+    """The device tensors of a dataclass, looked at once: `_at[name]` is (address, entries, device)."""
+    _TYPES: dict = {}
+
+    def __post_init__(self):
+        object.__setattr__(self, "_at", {f.name: _flat(getattr(self, f.name), f.name, self._TYPES.get(f.name, "torch.int32")) for f in fields(self)})
+
+    def _ptr(self, dev: Device, name: str, n: int):
+        at, entries, where = self._at[name]
+        if at is not None and (entries < n or where != dev.ordinal):
+            _at(dev, name, n, entries, where)
+        return at
 
 
 @dataclass
@@ -88,8 +122,9 @@ class Rotary:
             _need(t.dim() == 2 and str(t.dtype) == "torch.float32" and t.is_contiguous() and t.is_cuda and t.shape == cos.shape, _ffi.FC_ERR_ARG,
                   f"{name} must be a contiguous float32 [positions, rope_dim / 2] tensor on the device")
         self.cos, self.sin = cos, sin
-        self._c = _ffi.FcRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
-                                _ffi.FC_ROPE_NEOX if neox else _ffi.FC_ROPE_NORM)
+        c = _ffi.FcRotary(cos.data_ptr(), sin.data_ptr(), cos.shape[0], 2 * cos.shape[1],
+                          _ffi.FC_ROPE_NEOX if neox else _ffi.FC_ROPE_NORM)
+        self._ref = C.byref(c)
 
     @classmethod
     def build(cls, dev: Device, scaling: RopeScaling, positions: int, neox: bool) -> "Rotary":
@@ -99,15 +134,16 @@ class Rotary:
         return cls(cos, sin, neox)
 
 
-@dataclass
-class Step:
-    """The rows of one step. `extend` fills all of it; `append` reads slot and position, `attend` position and request.
+@dataclass(frozen=True)
+class Step(_Buffers):
+    """The rows of one step: buffers that a program keeps from step to step. `extend` fills all of it; `append` reads slot and position, `attend` position and request.
     Rows past the step's tokens have -1 everywhere."""
     starts: Any = None    # int32 [requests of the step + 1]: each one's first row, and the total
     slot: Any = None      # int64 [rows]
     position: Any = None  # int32 [rows]
     request: Any = None   # int32 [rows]: the row of the page table
     status: Any = None    # int32 [1]: 0, the number of pages that are missing, or an FC_ERR_* code
+    _TYPES = {"slot": "torch.int64"}
 
     @classmethod
     def new(cls, dev: Device, requests: int, rows: int) -> "Step":
@@ -136,12 +172,14 @@ class PagedCache:
         requests, most = (0, 0) if table is None else table.shape
         pages = self.layers[0][0].shape[0] if self.layers else free.numel() if free is not None else 0
         _need(free is None or free.numel() == pages, _ffi.FC_ERR_SHAPE, "the stack of free pages has another length than the pool")
-        self._plan = (_ints(dev, table, "table"), _ints(dev, lens, "lens", requests), _ints(dev, free, "free"), _ints(dev, n_free, "n_free", 1))
+        self._requests = requests
+        plan = (_ints(dev, table, "table"), _ints(dev, lens, "lens", requests), _ints(dev, free, "free"), _ints(dev, n_free, "n_free", 1))
         self._views = []
         for k, v in self.layers or [(None, None)]:
             kv_heads, head_dim, kind = (0, 0, 0) if k is None else (k.shape[1], k.shape[3], _kind(k))
             self._views.append(_ffi.FcPagedCache(page, pages, kv_heads, head_dim, kind, None if k is None else k.data_ptr(),
-                                                 None if v is None else v.data_ptr(), requests, most, *self._plan))
+                                                 None if v is None else v.data_ptr(), requests, most, *plan))
+        self._refs = [C.byref(v) for v in self._views]
 
     @classmethod
     def new(cls, dev: Device, layers: int, kv_heads: int, head_dim: int, pages: int, page: int, requests: int, max_pages: int,
@@ -160,23 +198,20 @@ class PagedCache:
         """Pages, slots and positions of the step's tokens: request `requests[i]` (a row of the table; None: i) grows by
         `grow[i]` tokens. All or nothing: see `Step.status`. Lengths and stack height change in place unless others are given."""
         dev, n = self.dev, grow.numel()
-        rows = {t.numel() for t in (step.slot, step.position, step.request) if t is not None}
+        rows = {step._at[name][1] for name in ("slot", "position", "request")} - {None}
         _need(len(rows) <= 1, _ffi.FC_ERR_SHAPE, "slot, position and request of a step must have one length")
+        rows = rows.pop() if rows else 0
         dev.check(self._lib.fc_paged_extend_dev(
-            dev.handle, C.byref(self._views[0]), _ints(dev, requests, "requests", n), _ints(dev, grow, "grow"), n, rows.pop() if rows else 0,
-            _ints(dev, step.starts, "starts", n + 1), _ints(dev, step.slot, "slot", dtype="torch.int64"), _ints(dev, step.position, "position"),
-            _ints(dev, step.request, "request"), self._lens_out(lens_out), _ints(dev, n_free_out, "n_free_out", 1),
-            _ints(dev, step.status, "status", 1)))
+            dev.handle, self._refs[0], _ints(dev, requests, "requests", n), _ints(dev, grow, "grow"), n, rows, step._ptr(dev, "starts", n + 1),
+            step._ptr(dev, "slot", rows), step._ptr(dev, "position", rows), step._ptr(dev, "request", rows),
+            _ints(dev, lens_out, "lens_out", self._requests), _ints(dev, n_free_out, "n_free_out", 1), step._ptr(dev, "status", 1)))
 
     def release(self, requests, status, lens_out=None, n_free_out=None):
         """All pages of these requests back onto the stack, their lengths 0."""
         dev = self.dev
-        dev.check(self._lib.fc_paged_release_dev(dev.handle, C.byref(self._views[0]), _ints(dev, requests, "requests"), requests.numel(),
-                                                 self._lens_out(lens_out), _ints(dev, n_free_out, "n_free_out", 1),
-                                                 _ints(dev, status, "status", 1)))
-
-    def _lens_out(self, t):
-        return _ints(self.dev, t, "lens_out", 0 if self.table is None else self.table.shape[0])
+        dev.check(self._lib.fc_paged_release_dev(
+            dev.handle, self._refs[0], _ints(dev, requests, "requests"), requests.numel(), _ints(dev, lens_out, "lens_out", self._requests),
+            _ints(dev, n_free_out, "n_free_out", 1), _ints(dev, status, "status", 1)))
 
     def append(self, layer: int, qkv, step: Step, q_out, rotary: Rotary | None = None):
         """Rows q heads | k heads | v heads: q and k rotated by `rotary` (None: not), q to the rows of `q_out`, k and v to the
@@ -187,11 +222,12 @@ class PagedCache:
         rows, width = qkv.shape
         hd, kv = view.head_dim, view.kv_heads
         heads = width // hd - 2 * kv
-        _need(width % hd == 0 and heads > 0, _ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {hd} beside {2 * kv}")
-        _need(q_kind == kind and tuple(q_out.shape) == (rows, heads * hd), _ffi.FC_ERR_SHAPE, f"q_out must be {rows} x {heads * hd} of qkv's type")
-        dev.check(self._lib.fc_paged_append_dev(dev.handle, C.byref(view), C.byref(rotary._c) if rotary is not None else None, at, kind, stride,
-                                                rows, heads, _ints(dev, step.slot, "slot", rows, "torch.int64"),
-                                                _ints(dev, step.position, "position", rows), q_at, q_stride))
+        if width % hd or heads <= 0:
+            raise CudaError(_ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {hd} beside {2 * kv}")
+        if q_kind != kind or q_out.shape != (rows, heads * hd):
+            raise CudaError(_ffi.FC_ERR_SHAPE, f"q_out must be {rows} x {heads * hd} of qkv's type")
+        dev.check(self._lib.fc_paged_append_dev(dev.handle, self._refs[layer], rotary._ref if rotary is not None else None, at, kind, stride, rows,
+                                                heads, step._ptr(dev, "slot", rows), step._ptr(dev, "position", rows), q_at, q_stride))
 
     def attend(self, layer: int, q, step: Step, out, scale: float = 0.0):
         """Every row of `q` over positions 0 .. position of its request; `scale` 0 is 1 / sqrt(head_dim)."""
@@ -199,25 +235,34 @@ class PagedCache:
         at, kind, stride = _rows(dev, q, "q")
         out_at, out_kind, out_stride = _rows(dev, out, "out")
         rows, width = q.shape
-        _need(width % view.head_dim == 0, _ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {view.head_dim}")
-        _need(out_kind == kind and out.shape == q.shape, _ffi.FC_ERR_SHAPE, "the result must have q's shape and type")
-        dev.check(self._lib.fc_paged_attend_dev(dev.handle, C.byref(view), at, kind, stride, rows, width // view.head_dim,
-                                                _ints(dev, step.request, "request", rows), _ints(dev, step.position, "position", rows),
-                                                float(scale), out_at, out_stride))
+        if width % view.head_dim:
+            raise CudaError(_ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {view.head_dim}")
+        if out_kind != kind or out.shape != q.shape:
+            raise CudaError(_ffi.FC_ERR_SHAPE, "the result must have q's shape and type")
+        dev.check(self._lib.fc_paged_attend_dev(dev.handle, self._refs[layer], at, kind, stride, rows, width // view.head_dim,
+                                                step._ptr(dev, "request", rows), step._ptr(dev, "position", rows), scale, out_at, out_stride))
 
     def _view(self, layer: int):
-        _need(self.layers and 0 <= layer < len(self.layers), _ffi.FC_ERR_RANGE, f"layer {layer} of {len(self.layers)}")
+        if not 0 <= layer < len(self.layers):
+            raise CudaError(_ffi.FC_ERR_RANGE, f"layer {layer} of {len(self.layers)}")
         return self._views[layer]
 
 
-@dataclass
-class LogProbs:
+@dataclass(frozen=True)
+class LogProbs(_Buffers):
     """Where `logprobs` puts its results; what is None is not computed."""
     logprob: Any = None      # f32 [rows]: of the target; NaN where there is none
     entropy: Any = None      # f32 [rows], nats
     rank: Any = None         # int32 [rows]: 0 is the greedy pick; -1 where there is no target
     top_index: Any = None    # int32 [rows, top]
     top_logprob: Any = None  # f32 [rows, top]
+    _TYPES = {"logprob": "torch.float32", "entropy": "torch.float32", "top_logprob": "torch.float32"}
+
+    def __post_init__(self):
+        super().__post_init__()
+        tops = {tuple(t.shape) for t in (self.top_index, self.top_logprob) if t is not None}
+        _need(len(tops) <= 1 and all(len(s) == 2 for s in tops), _ffi.FC_ERR_SHAPE, "the alternatives must be rows of one width")
+        object.__setattr__(self, "_top", tops.pop() if tops else None)
 
     @classmethod
     def new(cls, dev: Device, rows: int, top: int) -> "LogProbs":
@@ -232,13 +277,13 @@ class LogProbs:
 def logprobs(dev: Device, logits, targets, out: LogProbs, vocab: int | None = None):
     """Log-probability and rank of `targets` (int32 [rows], -1: none; None: nowhere), entropy and the largest alternatives of
     the first `vocab` elements (None: all) of every row of `logits`."""
-    lib = _ffi.load()
     at, kind, stride = _rows(dev, logits, "logits")
     rows, width = logits.shape
-    _need(vocab is None or 0 < vocab <= width, _ffi.FC_ERR_SHAPE, f"{vocab} logits of rows of {width}")
-    tops = {tuple(t.shape) for t in (out.top_index, out.top_logprob) if t is not None}
-    _need(len(tops) <= 1 and all(len(s) == 2 and s[0] == rows for s in tops), _ffi.FC_ERR_SHAPE, f"the alternatives must be {rows} rows of one width")
-    dev.check(lib.fc_logprobs_dev(dev.handle, at, kind, rows, stride, width if vocab is None else vocab, _ints(dev, targets, "targets", rows),
-                                  tops.pop()[1] if tops else 0, _ints(dev, out.logprob, "logprob", rows, "torch.float32"),
-                                  _ints(dev, out.entropy, "entropy", rows, "torch.float32"), _ints(dev, out.rank, "rank", rows),
-                                  _ints(dev, out.top_index, "top_index"), _ints(dev, out.top_logprob, "top_logprob", dtype="torch.float32")))
+    if vocab is not None and not 0 < vocab <= width:
+        raise CudaError(_ffi.FC_ERR_SHAPE, f"{vocab} logits of rows of {width}")
+    top = out._top[1] if out._top else 0
+    n = rows * top
+    dev.check(_ffi.load().fc_logprobs_dev(
+        dev.handle, at, kind, rows, stride, width if vocab is None else vocab, _ints(dev, targets, "targets", rows), top,
+        out._ptr(dev, "logprob", rows), out._ptr(dev, "entropy", rows), out._ptr(dev, "rank", rows), out._ptr(dev, "top_index", n),
+        out._ptr(dev, "top_logprob", n)))

@@ -191,7 +191,9 @@ def test_refusals(dev):
     refused(_ffi.FC_ERR_UNSUPPORTED, "at most 32", x, None, LogProbs.new(dev, 2, 33))
     refused(_ffi.FC_ERR_UNSUPPORTED, "float32", x.double(), None, out)
     refused(_ffi.FC_ERR_SHAPE, "has 1 entries, needs 2", x, torch.zeros(1, dtype=torch.int32, device="cuda"), out)
-    refused(_ffi.FC_ERR_SHAPE, "one width", x, None, LogProbs(top_index=out.top_index, top_logprob=LogProbs.new(dev, 2, 4).top_logprob))
+    refused(_ffi.FC_ERR_SHAPE, "logprob has 1 entries, needs 2", x, None, LogProbs.new(dev, 1, 3))
+    with pytest.raises(CudaError, match="one width"):
+        LogProbs(top_index=out.top_index, top_logprob=LogProbs.new(dev, 2, 4).top_logprob)
     refused(_ffi.FC_ERR_ARG, "side by side", x.T, None, out)
     refused(_ffi.FC_ERR_ARG, "contiguous torch.int32", x, torch.zeros(2, dtype=torch.int64, device="cuda"), out)
     refused(_ffi.FC_ERR_SHAPE, "rows of 64 logits 3 apart", torch.as_strided(x, (2, 64), (3, 1)), None, out)

@@ -493,7 +493,7 @@ def test_refusals(dev):
     refused(R, "5 rows in a table of 3", cache.attend, 0, q, Step(position=step.position), out)
     refused(A, "page table", PagedCache(dev, 16, layers=kv).attend, 0, q, step, out)
     refused(R, "layer 1 of 1", cache.attend, 1, q, step, out)
-    refused(A, "contiguous torch.int32", cache.attend, 0, q, Step(position=step.position.long(), request=step.request), out)
+    refused(A, "contiguous torch.int32", Step, position=step.position.long(), request=step.request)
     refused(A, "on cuda", cache.attend, 0, q.cpu(), step, out)
     qkv = f(5, 512, device="cuda")
     refused(S, "q_out must be", cache.append, 0, qkv, step, f(5, 255, device="cuda"))
