@@ -4,30 +4,37 @@
 // One pass with the softmax's running maximum and sum: where a later score raises the maximum from m to m', the sum and
 // the weighted values so far are multiplied by 2^(m - m') (scores are held times log2 e).
 //
-// What bounds it is the cache's bytes, so everything is laid out for reading them once, in 16-byte pieces, straight into the
-// registers that the matrix instructions take - no tile in shared memory, no copy between lanes:
-//  * mma.sync with the heads of a kv head as the 16 rows: 8 heads, each as two terms (row g the high one, row g + 8 the
-//    low one; q = high + low to 22 bits for f16 and tf32, 16 for bf16, where f32 rows bring a third term in a second
-//    instruction). The two partial results of a head end up in one thread and are added there.
+// What bounds it is the cache's bytes. One warp of a CTA streams them into shared memory by TMA, tiles of 8 to 64 positions
+// (32 KB of k and v at 128 channels of 16 bits), as many ahead as the SM's shared memory holds; a box is one page's rows of
+// 128 bytes, swizzled; channels past head_dim arrive as zeros. Four warps multiply, on mma.sync:
+//  * the heads of a kv head are the 16 rows: 8 heads, each as two terms (row g the high one, row g + 8 the low one; q = high
+//    + low to 22 bits for f16 and tf32, 16 for bf16, where f32 rows bring a third term in a second instruction). The two
+//    partial results of a head end up in one thread and are added there.
 //  * scores: positions are the 8 columns, channels the depth. The order of channels along the depth is free as long as q has
-//    the same, so a lane takes the 16 consecutive bytes of its row that it can load at once.
+//    the same, so a lane reads 16 consecutive bytes of its row at once.
 //  * p v: positions are the depth - the scores' own layout is the layout of the first operand, no shuffle between the two
 //    products - and channels the columns, again in the order that 16-byte pieces of a position's row give.
+//  * Column c of a score is position spread(c) of its eight and column g of p v piece spread(g) of eight, spread moving the
+//    lowest bit to the top: with the swizzle, the eight lanes that read at once meet no bank twice.
 //  * an f32 cache goes as two tf32 terms (11 + 11 bits) made in registers.
 // p is at most 2^P_LIFT instead of 1 so that its low f16 term keeps its bits far below the maximum.
 //
-// Work: tiles of 64 positions of (row, kv head, 8 heads), all of a step in one line, cut evenly over the CTAs that are
-// resident at once: a row alone is spread over the GPU, rows of unequal length cost what they hold. A CTA's four warps take
-// 16 positions in turn and join through shared memory; a (row, kv head) that several CTAs share is joined by the one
-// that arrives last, from f32 partial results in the order of the positions - the same bits every time.
+// Work: tiles of (row, kv head, 8 heads), all of a step in one line, cut evenly over the CTAs that are resident at once: a
+// row alone is spread over the GPU, rows of unequal length cost what they hold. The four warps share a tile (or take tiles
+// in turn, where a tile has fewer positions than they need) and join through shared memory; a (row, kv head) that several
+// CTAs share is joined by the one that arrives last, from f32 partial results in the order of the positions - the same bits
+// every time.
 #include <cmath>
 #include <type_traits>
 
 #include "paged.cuh"
+#include "tc_ptx.cuh"
+#include "tensor_map.cuh"
 
 namespace {
 
-constexpr int WARPS = 4, TILE = 64, ROWS8 = 8; // warps of a CTA, positions of a tile, heads of one matrix operand
+constexpr int WARPS = 4, ROWS8 = 8; // multiplying warps of a CTA (one more loads), heads of one matrix operand
+constexpr int THREADS = WARPS * 32 + 32;
 constexpr float P_LIFT = 10.0f;
 
 struct AttendArgs {
@@ -40,6 +47,7 @@ struct AttendArgs {
   float scale; // times log2 e
   float* parts;
   uint32_t* arrived;
+  int* err_flag;
 };
 // a part: 8 maxima, 8 sums, 8 rows of weighted values
 constexpr uint32_t part_floats(uint32_t hdp) { return 2 * ROWS8 + ROWS8 * hdp; }
@@ -91,7 +99,19 @@ __device__ __forceinline__ uint32_t take_term<__nv_bfloat16>(float& x, float& y)
   x -= f.x, y -= f.y;
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ uint4 load16(const char* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+               "l"(tmap), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
+__device__ __forceinline__ void warps_sync() { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); } // the multiplying warps
+// the lowest of three bits to the top
+__device__ __forceinline__ uint32_t spread(uint32_t c) { return (c & 1) << 2 | c >> 1; }
 __device__ __forceinline__ float load_act(const void* p, int act, size_t i) {
   return act == FC_F32 ? static_cast<const float*>(p)[i] : act == FC_F16 ? to_f32(static_cast<const __half*>(p)[i]) : to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
 }
@@ -109,36 +129,73 @@ __device__ __forceinline__ uint32_t row_len(const AttendArgs& a, uint32_t r, uin
   const uint64_t cap = (uint64_t)a.max_pages << a.page_shift;
   return ok ? (uint32_t)min((uint64_t)p + 1, cap) : 0u;
 }
-__device__ __forceinline__ uint32_t row_tiles(uint32_t len) { return max(1u, (len + TILE - 1) / TILE); }
+// What a kernel's shared memory holds. HDP: head_dim rounded up to what the registers are laid out for.
+template <typename C, int HDP>
+struct Shape {
+  static constexpr bool F32 = sizeof(C) == 4;
+  static constexpr int E = 16 / sizeof(C);                               // elements of a 16-byte piece
+  static constexpr int BOXES = HDP * (int)sizeof(C) / 128;               // boxes of 128 bytes across a row
+  static constexpr int TP = HDP == 256 ? (F32 ? 8 : 16) : F32 && HDP == 128 ? 32 : 64; // positions of a tile
+  static constexpr int PS = F32 && HDP > 64 ? 8 : 16;                    // positions of a warp's step
+  static constexpr int SHARE = TP / PS, GROUPS = WARPS / SHARE;          // warps that share a tile; groups that take tiles in turn
+  static constexpr uint32_t HALF = TP * BOXES * 128, STAGE = 2 * HALF;   // bytes of k (or v), of both
+  static constexpr int CTAS = HDP == 64 && !F32 ? 3 : 2;                 // resident on an SM
+  static constexpr int STAGES = HDP == 256 ? 5 : HDP == 64 && !F32 ? 4 : 3;
+  static constexpr uint32_t Q_BYTES = HDP / (4 * E) * 3 * 32 * 16, JOIN_BYTES = 2 * ROWS8 * HDP * 4;
+  static constexpr uint32_t SHARED = STAGES * STAGE + (Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES);
+  static constexpr uint32_t BYTES = SHARED + 1024; // (tiles begin on whole swizzle patterns)
+};
 
-// HDP: channels rounded up to what the registers are laid out for; FULL: head_dim is HDP; TERMS: of q and p (bf16: 2 or 3)
-template <typename C, int HDP, bool FULL, int TERMS>
-__global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(AttendArgs a) {
-  constexpr bool F32 = sizeof(C) == 4;
-  constexpr int E = 16 / sizeof(C);             // elements of a 16-byte piece
-  constexpr int NJ = HDP / (4 * E);             // pieces of a k row per lane (4 lanes share a row)
-  constexpr int NI = HDP / (8 * E);             // pieces of a v row per lane (8 lanes share a row)
-  constexpr int PS = F32 && HDP > 64 ? 8 : 16;  // positions of a warp's step
-  constexpr int NT = PS / 8;
+// A CTA's walk over its tiles: the same in the warp that loads and in those that multiply.
+struct Walk {
+  uint32_t r, req, len, tiles, row_at, which, tile, at;
+};
+template <int TP>
+__device__ __forceinline__ uint32_t row_tiles(uint32_t len) {
+  return max(1u, (len + TP - 1) / TP);
+}
+template <int TP>
+__device__ __forceinline__ void next_segment(const AttendArgs& a, uint32_t per_row, uint32_t tile_end, Walk& w) {
+  w.at += tile_end - w.tile;
+  w.tile = 0;
+  if (tile_end == w.tiles && ++w.which == per_row) {
+    w.row_at += w.tiles * per_row;
+    w.which = 0;
+    if (++w.r < a.rows) w.len = row_len(a, w.r, w.req), w.tiles = row_tiles<TP>(w.len);
+  }
+}
+
+template <typename C, int HDP, int TERMS>
+__global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
+    attend_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, AttendArgs a) {
+  using S = Shape<C, HDP>;
+  constexpr bool F32 = S::F32;
+  constexpr int E = S::E, TP = S::TP, PS = S::PS, NT = PS / 8, STAGES = S::STAGES;
+  constexpr int NJ = HDP / (4 * E); // pieces of a k row per lane (4 lanes share a row)
+  constexpr int NI = HDP / (8 * E); // pieces of a v row per lane (8 lanes share a row)
   constexpr bool SIZED = std::is_same<C, __half>::value; // its terms have a range to keep to
-  constexpr bool AHEAD = HDP <= 128;            // the next step's k is requested before this one's softmax
-  __shared__ union { // q while positions are multiplied, then the warps' results
-    uint4 q[NJ][TERMS][32];
-    float o[WARPS][ROWS8][HDP];
-  } sm;
-  auto& sm_q = sm.q;
-  auto& sm_o = sm.o;
+  extern __shared__ char raw[];
   __shared__ float sm_m[WARPS][ROWS8], sm_l[WARPS][ROWS8];
   __shared__ uint32_t sm_big[ROWS8];
-  __shared__ uint32_t sm_scan[WARPS], sm_row, sm_at, sm_last;
-  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  __shared__ uint32_t sm_scan[WARPS + 1], sm_row, sm_at, sm_last;
+  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ unsigned long long held[STAGES]; // of a tile: which of its pages are pages
+  const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t stages = (tc::smem_u32(raw) + 1023) & ~1023u;
+  char* shared = raw + (stages - tc::smem_u32(raw)) + STAGES * S::STAGE;
+  uint4 (*sm_q)[3][32] = reinterpret_cast<uint4 (*)[3][32]>(shared);      // q's terms while positions are multiplied,
+  float (*sm_o)[ROWS8][HDP] = reinterpret_cast<float (*)[ROWS8][HDP]>(shared); // then what two warps hand to the others
   const uint32_t per_row = a.kv_heads * a.blocks;
+  if (tid == 0) {
+    for (int s = 0; s < STAGES; s++) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], S::SHARE);
+    tc::fence_barrier_init();
+  }
   grid_wait();
 
   // Where this CTA's share of the tiles begins: prefix sums over the rows' tiles, a run of rows per thread.
-  const uint32_t run = (a.rows + WARPS * 32 - 1) / (WARPS * 32), r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
+  const uint32_t run = (a.rows + THREADS - 1) / THREADS, r0 = min(a.rows, tid * run), r1 = min(a.rows, r0 + run);
   uint32_t mine = 0, req;
-  for (uint32_t r = r0; r < r1; r++) mine += row_tiles(row_len(a, r, req));
+  for (uint32_t r = r0; r < r1; r++) mine += row_tiles<TP>(row_len(a, r, req));
   uint32_t upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -149,7 +206,7 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
   __syncthreads();
   uint32_t all = 0;
 #pragma unroll
-  for (int w = 0; w < WARPS; w++) {
+  for (int w = 0; w <= WARPS; w++) {
     if (w < (int)warp) upto += sm_scan[w];
     all += sm_scan[w];
   }
@@ -157,34 +214,97 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
   const uint32_t n_cta = min(gridDim.x, all), share = all / n_cta, extra = all % n_cta; // (the first `extra` CTAs take one more)
   if (blockIdx.x >= n_cta) return;
   auto begin_of = [&](uint32_t c) { return c * share + min(c, extra); };
-  auto owner_of = [&](uint32_t tile) {
-    const uint32_t longer = extra * (share + 1);
-    return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
-  };
   const uint32_t begin = begin_of(blockIdx.x), end = begin_of(blockIdx.x + 1);
   if (upto - mine <= begin && begin < upto) {
     uint32_t at = upto - mine, r = r0;
     for (;; r++) {
-      const uint32_t n = row_tiles(row_len(a, r, req)) * per_row;
+      const uint32_t n = row_tiles<TP>(row_len(a, r, req)) * per_row;
       if (begin < at + n) break;
       at += n;
     }
     sm_row = r, sm_at = at;
   }
   __syncthreads();
-  uint32_t r = sm_row, len = row_len(a, r, req), tiles = row_tiles(len);
-  uint32_t row_at = sm_at; // the row's first tile
-  uint32_t which = (begin - row_at) / tiles, tile = (begin - row_at) % tiles;
+  Walk w;
+  w.r = sm_row, w.len = row_len(a, w.r, w.req), w.tiles = row_tiles<TP>(w.len), w.row_at = sm_at;
+  w.which = (begin - w.row_at) / w.tiles, w.tile = (begin - w.row_at) % w.tiles, w.at = begin;
 
-  const size_t row_bytes = (size_t)a.hd * sizeof(C);
-  for (uint32_t at = begin; at < end;) {
-    const uint32_t tile_end = min(tiles, tile + (end - at));
-    const uint32_t kvh = which / a.blocks, h0 = kvh * a.group + (which % a.blocks) * ROWS8;
+  if (warp == WARPS) {
+    // ---- the loading warp: lane i loads page i of the tile (pages of one position in tiles of 64: also i + 32) ----
+    constexpr uint32_t TP_SHIFT = TP == 64 ? 6 : TP == 32 ? 5 : TP == 16 ? 4 : 3;
+    const uint32_t box_shift = min(a.page_shift, TP_SHIFT), mask = (1u << a.page_shift) - 1;
+    uint32_t stage = 0, phase = 0, n = 0;
+    bool alive = true;
+    auto look = [&](const Walk& w, uint32_t i) { // the page of the i-th box of w's tile
+      const uint32_t p = w.tile * TP + (i << box_shift);
+      return w.at < end && i < (TP >> box_shift) && p < w.len ? (uint32_t)a.table[(size_t)w.req * a.max_pages + (p >> a.page_shift)] : 0u;
+    };
+    uint32_t page0 = look(w, lane), page1 = TP > 32 ? look(w, lane + 32) : 0;
+    while (w.at < end) {
+      Walk ahead = w; // the next tile's pages are looked up before this one's turn comes
+      if (++ahead.tile == ahead.tiles) {
+        ahead.tile--;
+        next_segment<TP>(a, per_row, ahead.tiles, ahead);
+      } else {
+        ahead.at++;
+      }
+      const uint32_t next0 = look(ahead, lane), next1 = TP > 32 ? look(ahead, lane + 32) : 0;
+      const uint32_t here = w.len > w.tile * TP ? min((uint32_t)TP, w.len - w.tile * TP) : 0u;
+      const uint32_t boxes = (here + (1u << box_shift) - 1) >> box_shift; // pages with positions of the tile
+      const uint32_t ok0 = __ballot_sync(0xffffffffu, lane >= boxes || page0 < a.n_pages);
+      const uint32_t ok1 = __ballot_sync(0xffffffffu, lane + 32 >= boxes || page1 < a.n_pages);
+      if (alive && n >= STAGES && !tc::mbar_wait(&empty[stage], phase ^ 1)) {
+        alive = false;
+        if (lane == 0) atomicExch(a.err_flag, 1);
+      }
+      __syncwarp();
+      if (lane == 0) {
+        held[stage] = (unsigned long long)ok1 << 32 | ok0;
+        tc::mbar_arrive_expect_tx(&full[stage], boxes * (128u << box_shift) * (2 * S::BOXES));
+      }
+      __syncwarp();
+      const uint32_t kvh = w.which / a.blocks;
+#pragma unroll
+      for (int half = 0; half < (TP > 32 ? 2 : 1); half++) {
+        const uint32_t i = lane + 32 * half;
+        if (i < boxes) {
+          const uint32_t p = w.tile * TP + (i << box_shift), page = half ? page1 : page0;
+          const int32_t y = (int32_t)((kvh << a.page_shift) + (p & mask)), z = page < a.n_pages ? (int32_t)page : 0; // (a page that is none: masked later)
+          const uint32_t dst = stages + stage * S::STAGE + (i << box_shift) * 128;
+#pragma unroll
+          for (int b = 0; b < S::BOXES; b++) {
+            tma_load_3d(dst + b * TP * 128, &map_k, &full[stage], b * (128 / (int)sizeof(C)), y, z);
+            tma_load_3d(dst + S::HALF + b * TP * 128, &map_v, &full[stage], b * (128 / (int)sizeof(C)), y, z);
+          }
+        }
+      }
+      if (++stage == STAGES) stage = 0, phase ^= 1;
+      n++, w = ahead, page0 = next0, page1 = next1;
+    }
+    // (no copy is in flight when the CTA ends, whatever became of the others' waits)
+    for (uint32_t i = 0; i < min(n, (uint32_t)STAGES); i++) {
+      if (stage == 0) stage = STAGES, phase ^= 1;
+      stage--;
+      if (!tc::mbar_wait(&full[stage], phase) && lane == 0) atomicExch(a.err_flag, 2);
+    }
+    return;
+  }
+
+  // ---- the multiplying warps ----
+  const uint32_t g = lane >> 2, t = lane & 3, sub = warp % S::SHARE, group = warp / S::SHARE;
+  // where this lane's pieces lie in a tile: row i of eight is swizzled by i
+  const uint32_t k_at = (sub * PS + spread(g)) * 128 + ((t ^ spread(g)) << 4);
+  const uint32_t v_at = S::HALF + (sub * PS + t) * 128 + ((spread(g) ^ t) << 4);
+  uint32_t stage = 0, phase = 0, turn = 0;
+  bool alive = true;
+  while (w.at < end) {
+    const uint32_t tile_end = min(w.tiles, w.tile + (end - w.at));
+    const uint32_t kvh = w.which / a.blocks, h0 = kvh * a.group + (w.which % a.blocks) * ROWS8;
     const uint32_t heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
     // q's terms as the matrix operand wants them: lane (g, t) of piece j has channels (4 j + t) E .. of head h0 + g
     if (SIZED) { // (the f16 terms of a head: of q divided by a power of two near its largest)
       if (tid < ROWS8) sm_big[tid] = 0;
-      __syncthreads();
+      warps_sync();
     }
     float mul = a.scale;
     constexpr int ITEMS = (NJ * 32 + WARPS * 32 - 1) / (WARPS * 32);
@@ -197,14 +317,14 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const uint32_t ch = (4 * j + t) * E + e;
-        qv[it][e] = g < heads && (FULL || ch < a.hd) ? load_act(a.q, a.act, (size_t)r * a.q_stride + (size_t)(h0 + g) * a.hd + ch) : 0.0f;
+        qv[it][e] = g < heads && ch < a.hd ? load_act(a.q, a.act, (size_t)w.r * a.q_stride + (size_t)(h0 + g) * a.hd + ch) : 0.0f;
         big = fmaxf(big, fabsf(qv[it][e]));
       }
       if (SIZED) atomicMax(&sm_big[g], __float_as_uint(big));
     }
     float down = 1.0f;
     if (SIZED) {
-      __syncthreads();
+      warps_sync();
       const int ex = min(max((int)(sm_big[g] >> 23), 27), 253) - 127; // (a power of two that has an inverse, whatever the largest is)
       down = __uint_as_float((uint32_t)(127 - ex) << 23), mul *= __uint_as_float((uint32_t)(127 + ex) << 23);
     }
@@ -212,25 +332,25 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
     for (int it = 0; it < ITEMS; it++) {
       const uint32_t id = tid + it * WARPS * 32, j = id / 32;
       if (NJ * 32 % (WARPS * 32) && id >= NJ * 32) continue;
-      uint32_t w[TERMS][4];
+      uint32_t q[TERMS][4];
       if constexpr (F32) {
 #pragma unroll
         for (int e = 0; e < E; e++) {
           const uint32_t x = __float_as_uint(qv[it][e]);
-          w[0][e] = tf32_high(x), w[1][e] = tf32_low(x, w[0][e]);
+          q[0][e] = tf32_high(x), q[1][e] = tf32_low(x, q[0][e]);
         }
       } else {
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
           float x = qv[it][e] * down, y = qv[it][e + 1] * down;
 #pragma unroll
-          for (int m = 0; m < TERMS; m++) w[m][e / 2] = take_term<C>(x, y);
+          for (int m = 0; m < TERMS; m++) q[m][e / 2] = take_term<C>(x, y);
         }
       }
 #pragma unroll
-      for (int m = 0; m < TERMS; m++) sm_q[j][m][lane] = make_uint4(w[m][0], w[m][1], w[m][2], w[m][3]);
+      for (int m = 0; m < TERMS; m++) sm_q[j][m][lane] = make_uint4(q[m][0], q[m][1], q[m][2], q[m][3]);
     }
-    __syncthreads();
+    warps_sync();
 
     float o[NI][E][4], top = -INFINITY, sum = 0.0f; // of head g: the maximum is the lane's four's, the sum its own positions'
 #pragma unroll
@@ -240,206 +360,233 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
 #pragma unroll
         for (int c = 0; c < 4; c++) o[i][e][c] = 0.0f;
 
-    const uint32_t p_end = min(len, tile_end * TILE), mask = (1u << a.page_shift) - 1;
-    const int32_t* table = a.table + (size_t)req * a.max_pages;
-    const uint64_t page_rows = (uint64_t)a.kv_heads << a.page_shift, head_row = (uint64_t)kvh << a.page_shift;
-    // the page of position p + lane (mod the step's), none past the end
-    auto look = [&](uint32_t p) {
-      const uint32_t pos = p + (lane & (PS - 1));
-      const uint32_t page = pos < p_end ? (uint32_t)table[pos >> a.page_shift] : 0xffffffffu;
-      return page < a.n_pages ? page : 0xffffffffu;
-    };
-    auto row_of = [&](uint32_t page, uint32_t pos) { // (a page that is none: the pool's first, to be masked)
-      return ((page == 0xffffffffu ? 0 : page) * page_rows + head_row + (pos & mask)) * row_bytes;
-    };
-    uint4 kk[NT][NJ];
-    auto load_k = [&](uint32_t p, uint32_t pages) {
-#pragma unroll
-      for (int n = 0; n < NT; n++) {
-        const uint32_t i = n * 8 + g;
-        const char* src = static_cast<const char*>(a.k) + row_of(__shfl_sync(0xffffffffu, pages, i), p + i) + t * 16;
-#pragma unroll
-        for (int j = 0; j < NJ; j++) kk[n][j] = FULL || (4 * j + t) * E < a.hd ? load16(src + j * 64) : make_uint4(0, 0, 0, 0);
+    for (uint32_t tile = w.tile; tile < tile_end; tile++) {
+      const uint32_t now = stage, ph = phase;
+      if (++stage == STAGES) stage = 0, phase ^= 1;
+      if (S::GROUPS > 1) {
+        const bool ours = turn == group;
+        turn = turn + 1 == S::GROUPS ? 0 : turn + 1;
+        if (!ours) continue;
       }
-    };
-    uint32_t p = tile * TILE + warp * PS;
-    uint32_t pages = look(p), pages_next = look(p + WARPS * PS);
-    if (AHEAD && p < p_end) load_k(p, pages);
-    for (; p < p_end; p += WARPS * PS) {
-      if (!AHEAD) load_k(p, pages);
-      uint4 vv[NT][2][NI];
-      bool ok[NT][2];
-      bool clean = true;
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const uint32_t i = n * 8 + 2 * t + x, page = __shfl_sync(0xffffffffu, pages, i);
-          ok[n][x] = page != 0xffffffffu;
-          clean = clean && ok[n][x];
-          const char* src = static_cast<const char*>(a.v) + row_of(page, p + i) + g * 16;
-#pragma unroll
-          for (int c = 0; c < NI; c++) vv[n][x][c] = FULL || (8 * c + g) * E < a.hd ? load16(src + c * 128) : make_uint4(0, 0, 0, 0);
-        }
-      float s[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) s[n][c] = 0.0f;
-#pragma unroll
-      for (int j = 0; j < NJ; j++) {
-        const uint4 hi = sm_q[j][0][lane], lo = sm_q[j][1][lane];
-        const uint32_t a0[4] = {hi.x, lo.x, hi.y, lo.y}, a1[4] = {hi.z, lo.z, hi.w, lo.w};
-        if constexpr (F32) {
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            const uint32_t k0 = tf32_high(kk[n][j].x), k1 = tf32_high(kk[n][j].y), k2 = tf32_high(kk[n][j].z), k3 = tf32_high(kk[n][j].w);
-            mma<C>(s[n], a0, k0, k1);
-            mma<C>(s[n], a1, k2, k3);
-            mma<C>(s[n], a0, tf32_low(kk[n][j].x, k0), tf32_low(kk[n][j].y, k1));
-            mma<C>(s[n], a1, tf32_low(kk[n][j].z, k2), tf32_low(kk[n][j].w, k3));
-          }
-        } else {
-#pragma unroll
-          for (int n = 0; n < NT; n++) {
-            mma<C>(s[n], a0, kk[n][j].x, kk[n][j].y);
-            mma<C>(s[n], a1, kk[n][j].z, kk[n][j].w);
-          }
-          if constexpr (TERMS == 3) {
-            const uint4 ll = sm_q[j][TERMS - 1][lane];
-            const uint32_t b0[4] = {ll.x, 0, ll.y, 0}, b1[4] = {ll.z, 0, ll.w, 0};
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-              mma<C>(s[n], b0, kk[n][j].x, kk[n][j].y);
-              mma<C>(s[n], b1, kk[n][j].z, kk[n][j].w);
-            }
-          }
-        }
+      if (alive && !tc::mbar_wait(&full[now], ph)) {
+        alive = false; // (reported; the results are wrong, the barriers stay whole)
+        if (lane == 0) atomicExch(a.err_flag, 3);
       }
-      pages = pages_next, pages_next = look(p + 2 * WARPS * PS);
-      if (AHEAD && p + WARPS * PS < p_end) load_k(p + WARPS * PS, pages);
-      clean = __all_sync(0xffffffffu, clean);
-      float best = -INFINITY;
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) {
-          const float v = (s[n][x] + s[n][x + 2]) * mul;
-          s[n][x] = clean || ok[n][x] ? v : -INFINITY;
-          best = fmaxf(best, s[n][x]);
-        }
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
-      best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
-      if (__any_sync(0xffffffffu, best > top)) {
-        const float higher = fmaxf(top, best), keep = higher == -INFINITY ? 1.0f : ex2(top - higher);
-        top = higher, sum *= keep;
-#pragma unroll
-        for (int i = 0; i < NI; i++)
-#pragma unroll
-          for (int e = 0; e < E; e++)
-#pragma unroll
-            for (int c = 0; c < 4; c++) o[i][e][c] *= keep; // (rows g and g + 8 are one head)
-      }
-      const float base = top == -INFINITY ? 0.0f : top - P_LIFT;
-      float pr[NT][2];
-#pragma unroll
-      for (int n = 0; n < NT; n++)
-#pragma unroll
-        for (int x = 0; x < 2; x++) pr[n][x] = ex2(s[n][x] - base), sum += pr[n][x];
-      if (!clean) { // what no position holds may be NaN, and 0 * NaN is not 0
+      const uint32_t p = tile * TP + sub * PS;
+      if (p < w.len) {
+        const uint32_t base_at = stages + now * S::STAGE;
+        float s[NT][4];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int x = 0; x < 2; x++)
-            if (!ok[n][x])
+          for (int c = 0; c < 4; c++) s[n][c] = 0.0f;
 #pragma unroll
-              for (int c = 0; c < NI; c++) vv[n][x][c] = make_uint4(0, 0, 0, 0);
-      }
-      if constexpr (F32) {
+        for (int j = 0; j < NJ; j++) {
+          const uint4 hi = sm_q[j][0][lane], lo = sm_q[j][1][lane];
+          const uint32_t a0[4] = {hi.x, lo.x, hi.y, lo.y}, a1[4] = {hi.z, lo.z, hi.w, lo.w};
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-          const uint32_t x = __float_as_uint(pr[n][0]), y = __float_as_uint(pr[n][1]), xh = tf32_high(x), yh = tf32_high(y);
-          const uint32_t pa[4] = {xh, tf32_low(x, xh), yh, tf32_low(y, yh)};
-#pragma unroll
-          for (int c = 0; c < NI; c++) {
-            const uint32_t u[4] = {vv[n][0][c].x, vv[n][0][c].y, vv[n][0][c].z, vv[n][0][c].w};
-            const uint32_t w[4] = {vv[n][1][c].x, vv[n][1][c].y, vv[n][1][c].z, vv[n][1][c].w};
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-              const uint32_t uh = tf32_high(u[e]), wh = tf32_high(w[e]);
-              mma<C>(o[c][e], pa, uh, wh);
-              mma<C>(o[c][e], pa, tf32_low(u[e], uh), tf32_low(w[e], wh));
+          for (int n = 0; n < NT; n++) {
+            const uint4 k = lds16(base_at + ((k_at + j / 2 * TP * 128 + n * 1024) ^ (j & 1) * 64));
+            if constexpr (F32) {
+              const uint32_t k0 = tf32_high(k.x), k1 = tf32_high(k.y), k2 = tf32_high(k.z), k3 = tf32_high(k.w);
+              mma<C>(s[n], a0, k0, k1);
+              mma<C>(s[n], a1, k2, k3);
+              mma<C>(s[n], a0, tf32_low(k.x, k0), tf32_low(k.y, k1));
+              mma<C>(s[n], a1, tf32_low(k.z, k2), tf32_low(k.w, k3));
+            } else {
+              mma<C>(s[n], a0, k.x, k.y);
+              mma<C>(s[n], a1, k.z, k.w);
+              if constexpr (TERMS == 3) {
+                const uint4 ll = sm_q[j][2][lane];
+                const uint32_t b0[4] = {ll.x, 0, ll.y, 0}, b1[4] = {ll.z, 0, ll.w, 0};
+                mma<C>(s[n], b0, k.x, k.y);
+                mma<C>(s[n], b1, k.z, k.w);
+              }
             }
           }
         }
-      } else {
-        uint32_t pa[4], pb[4];
-        pa[0] = take_term<C>(pr[0][0], pr[0][1]), pa[1] = take_term<C>(pr[0][0], pr[0][1]);
-        pa[2] = take_term<C>(pr[1][0], pr[1][1]), pa[3] = take_term<C>(pr[1][0], pr[1][1]);
-        if (TERMS == 3) pb[0] = take_term<C>(pr[0][0], pr[0][1]), pb[2] = take_term<C>(pr[1][0], pr[1][1]), pb[1] = pb[3] = 0;
+        // which of this lane's positions (8 n + 4 x + t of the step) there are
+        const unsigned long long pages = held[now];
+        const bool clean = pages == ~0ull && p + PS <= w.len;
+        uint32_t ok = ~0u;
+        if (!clean) {
+          ok = 0;
+#pragma unroll
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              const uint32_t i = sub * PS + n * 8 + x * 4 + t;
+              const uint32_t box = i >> a.page_shift; // (a page larger than the tile: 0)
+              if (tile * TP + i < w.len && (pages >> box & 1)) ok |= 1u << (2 * n + x);
+            }
+        }
+        float best = -INFINITY;
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) {
+            const float v = (s[n][x] + s[n][x + 2]) * mul;
+            s[n][x] = ok >> (2 * n + x) & 1 ? v : -INFINITY;
+            best = fmaxf(best, s[n][x]);
+          }
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 1));
+        best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, 2));
+        if (__any_sync(0xffffffffu, best > top)) {
+          const float higher = fmaxf(top, best), keep = higher == -INFINITY ? 1.0f : ex2(top - higher);
+          top = higher, sum *= keep;
+#pragma unroll
+          for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int e = 0; e < E; e++)
+#pragma unroll
+              for (int c = 0; c < 4; c++) o[i][e][c] *= keep; // (rows g and g + 8 are one head)
+        }
+        const float base = top == -INFINITY ? 0.0f : top - P_LIFT;
+        float pr[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+          for (int x = 0; x < 2; x++) pr[n][x] = ex2(s[n][x] - base), sum += pr[n][x];
+        uint32_t pa[NT][4], pb[4];
+        if constexpr (F32) {
+#pragma unroll
+          for (int n = 0; n < NT; n++) {
+            const uint32_t x = __float_as_uint(pr[n][0]), y = __float_as_uint(pr[n][1]);
+            pa[n][0] = tf32_high(x), pa[n][1] = tf32_low(x, pa[n][0]), pa[n][2] = tf32_high(y), pa[n][3] = tf32_low(y, pa[n][2]);
+          }
+        } else {
+          pa[0][0] = take_term<C>(pr[0][0], pr[0][1]), pa[0][1] = take_term<C>(pr[0][0], pr[0][1]);
+          pa[0][2] = take_term<C>(pr[1][0], pr[1][1]), pa[0][3] = take_term<C>(pr[1][0], pr[1][1]);
+          if (TERMS == 3) pb[0] = take_term<C>(pr[0][0], pr[0][1]), pb[2] = take_term<C>(pr[1][0], pr[1][1]), pb[1] = pb[3] = 0;
+        }
 #pragma unroll
         for (int c = 0; c < NI; c++) {
-          const uint32_t u[4][4] = {{vv[0][0][c].x, vv[0][0][c].y, vv[0][0][c].z, vv[0][0][c].w}, {vv[0][1][c].x, vv[0][1][c].y, vv[0][1][c].z, vv[0][1][c].w},
-                                    {vv[1][0][c].x, vv[1][0][c].y, vv[1][0][c].z, vv[1][0][c].w}, {vv[1][1][c].x, vv[1][1][c].y, vv[1][1][c].z, vv[1][1][c].w}};
+          uint4 v[NT][2];
 #pragma unroll
-          for (int e = 0; e < E; e++) {
-            const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
-            const uint32_t b0 = __byte_perm(u[0][e / 2], u[1][e / 2], pick), b1 = __byte_perm(u[2][e / 2], u[3][e / 2], pick);
-            mma<C>(o[c][e], pa, b0, b1);
-            if constexpr (TERMS == 3) mma<C>(o[c][e], pb, b0, b1);
+          for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+              v[n][x] = lds16(base_at + ((v_at + c * TP * 128 + n * 1024 + x * 512) ^ x * 64));
+              // what no position holds may be NaN, and 0 * NaN is not 0
+              if (!clean && !(ok >> (2 * n + x) & 1)) v[n][x] = make_uint4(0, 0, 0, 0);
+            }
+          if constexpr (F32) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+              const uint32_t u[4] = {v[n][0].x, v[n][0].y, v[n][0].z, v[n][0].w}, y[4] = {v[n][1].x, v[n][1].y, v[n][1].z, v[n][1].w};
+#pragma unroll
+              for (int e = 0; e < E; e++) {
+                const uint32_t uh = tf32_high(u[e]), yh = tf32_high(y[e]);
+                mma<C>(o[c][e], pa[n], uh, yh);
+                mma<C>(o[c][e], pa[n], tf32_low(u[e], uh), tf32_low(y[e], yh));
+              }
+            }
+          } else {
+            const uint32_t u[4][4] = {{v[0][0].x, v[0][0].y, v[0][0].z, v[0][0].w}, {v[0][1].x, v[0][1].y, v[0][1].z, v[0][1].w},
+                                      {v[1][0].x, v[1][0].y, v[1][0].z, v[1][0].w}, {v[1][1].x, v[1][1].y, v[1][1].z, v[1][1].w}};
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+              const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
+              const uint32_t b0 = __byte_perm(u[0][e / 2], u[1][e / 2], pick), b1 = __byte_perm(u[2][e / 2], u[3][e / 2], pick);
+              mma<C>(o[c][e], pa[0], b0, b1);
+              if constexpr (TERMS == 3) mma<C>(o[c][e], pb, b0, b1);
+            }
           }
         }
       }
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&empty[now]);
     }
 
-    // join the four warps
-    __syncthreads(); // (all have read q)
+    // join the four warps: 2 and 3 hand their results to 0 and 1, 1 to 0
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-    if (t == 0) sm_m[warp][g] = top, sm_l[warp][g] = sum;
 #pragma unroll
     for (int i = 0; i < NI; i++)
 #pragma unroll
-      for (int e = 0; e < E; e++)
+      for (int e = 0; e < E; e++) o[i][e][0] += o[i][e][2], o[i][e][1] += o[i][e][3];
+    warps_sync(); // (all have read q)
+    const uint32_t ch0 = t * E; // channels (8 i + 4 x + t) E + e of head g
+    auto give = [&](uint32_t buf) {
+      if (t == 0) sm_m[buf][g] = top, sm_l[buf][g] = sum;
 #pragma unroll
-        for (int x = 0; x < 2; x++) sm_o[warp][g][(8 * i + 2 * t + x) * E + e] = o[i][e][x] + o[i][e][x + 2];
-    __syncthreads();
-    const bool whole = tile == 0 && tile_end == tiles;
-    const uint32_t first_tile = row_at + which * tiles;
-    const uint32_t c0 = whole ? 0 : owner_of(first_tile), c1 = whole ? 0 : owner_of(first_tile + tiles - 1);
+      for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<float4*>(&sm_o[buf][g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
+    };
+    auto take = [&](uint32_t buf) {
+      const float m = sm_m[buf][g], higher = fmaxf(top, m), base = higher == -INFINITY ? 0.0f : higher;
+      const float mine = ex2(top - base), theirs = ex2(m - base);
+      top = higher, sum = fmaf(sum, mine, sm_l[buf][g] * theirs);
+#pragma unroll
+      for (int i = 0; i < NI; i++)
+#pragma unroll
+        for (int x = 0; x < 2; x++)
+#pragma unroll
+          for (int e = 0; e < E; e += 4) {
+            const float4 v = *reinterpret_cast<const float4*>(&sm_o[buf][g][(8 * i + 4 * x) * E + ch0 + e]);
+            o[i][e][x] = fmaf(o[i][e][x], mine, v.x * theirs), o[i][e + 1][x] = fmaf(o[i][e + 1][x], mine, v.y * theirs);
+            o[i][e + 2][x] = fmaf(o[i][e + 2][x], mine, v.z * theirs), o[i][e + 3][x] = fmaf(o[i][e + 3][x], mine, v.w * theirs);
+          }
+    };
+    if (warp >= 2) give(warp - 2);
+    warps_sync();
+    if (warp < 2) take(warp);
+    __syncwarp();
+    if (warp == 1) give(1);
+    warps_sync();
+    const bool whole = w.tile == 0 && tile_end == w.tiles;
+    const uint32_t first_tile = w.row_at + w.which * w.tiles;
     auto part_of = [&](uint32_t c) { // a CTA has two: one for where it begins, one for where it ends
       return a.parts + (size_t)(2 * c + (begin_of(c) >= first_tile ? 0 : 1)) * part_floats(HDP);
     };
-    float* part = whole ? nullptr : part_of(blockIdx.x);
-    for (uint32_t i = tid; i < heads * a.hd; i += WARPS * 32) {
-      const uint32_t h = i / a.hd, ch = i - h * a.hd;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < WARPS; w++) m = fmaxf(m, sm_m[w][h]);
-      const float base = m == -INFINITY ? 0.0f : m;
-      float l = 0.0f, v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < WARPS; w++) {
-        const float f = ex2(sm_m[w][h] - base);
-        l = fmaf(sm_l[w][h], f, l), v = fmaf(sm_o[w][h][ch], f, v);
-      }
+    if (warp == 0) {
+      take(1);
       if (whole) {
-        store_act(a.out, a.act, (size_t)r * a.out_stride + (size_t)(h0 + h) * a.hd + ch, l == 0.0f ? 0.0f : v / l);
+        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (g < heads) {
+          const size_t at = (size_t)w.r * a.out_stride + (size_t)(h0 + g) * a.hd;
+#pragma unroll
+          for (int i = 0; i < NI; i++)
+#pragma unroll
+            for (int x = 0; x < 2; x++)
+#pragma unroll
+              for (int e = 0; e < E; e++)
+                if ((8 * i + 4 * x) * E + ch0 + e < a.hd) store_act(a.out, a.act, at + (8 * i + 4 * x) * E + ch0 + e, o[i][e][x] * f);
+        }
       } else {
-        if (ch == 0) part[h] = m, part[ROWS8 + h] = l;
-        part[2 * ROWS8 + h * HDP + ch] = v;
+        float* part = part_of(blockIdx.x);
+        if (t == 0) part[g] = top, part[ROWS8 + g] = sum;
+#pragma unroll
+        for (int i = 0; i < NI; i++)
+#pragma unroll
+          for (int x = 0; x < 2; x++)
+#pragma unroll
+            for (int e = 0; e < E; e += 4)
+              *reinterpret_cast<float4*>(part + 2 * ROWS8 + g * HDP + (8 * i + 4 * x) * E + ch0 + e) =
+                  make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
       }
     }
     if (!whole) {
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) sm_last = atomicAdd(&a.arrived[c0], 1u) == c1 - c0;
-      __syncthreads();
+      auto owner_of = [&](uint32_t tile) {
+        const uint32_t longer = extra * (share + 1);
+        return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+      };
+      const uint32_t c0 = owner_of(first_tile), c1 = owner_of(first_tile + w.tiles - 1);
+      if (warp == 0) {
+        __threadfence();
+        __syncwarp();
+        if (lane == 0) sm_last = atomicAdd(&a.arrived[c0], 1u) == c1 - c0;
+      }
+      warps_sync();
       if (sm_last) {
         __threadfence();
         // Each warp finds two heads' maxima over the parts; then, JOIN parts at a time, their weights go to shared memory and
         // every thread adds its channels' values, all loads of a turn in flight together.
-        float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(&sm);
+        float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(shared);
         constexpr int JOIN = 32, OWN = (ROWS8 * HDP / 4 + WARPS * 32 - 1) / (WARPS * 32);
         {
           const uint32_t h = warp * 2 + (lane >> 4);
@@ -449,7 +596,7 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
           for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
           sm_m[0][h] = m == -INFINITY ? 0.0f : m; // (all lanes of a head write the same)
         }
-        __syncthreads();
+        warps_sync();
         float4 v[OWN];
         float l[OWN];
 #pragma unroll
@@ -462,11 +609,11 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
             const float f = ex2(__ldcg(q + h) - sm_m[0][h]);
             sm_w[i / ROWS8][h] = f, sm_w[JOIN + i / ROWS8][h] = f * __ldcg(q + ROWS8 + h);
           }
-          __syncthreads();
+          warps_sync();
 #pragma unroll
           for (int n = 0; n < OWN; n++) {
             const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
-            if (h >= heads || (!FULL && ch >= a.hd)) continue;
+            if (h >= heads || ch >= a.hd) continue;
             const float* q = a.parts + 2 * ROWS8 + h * HDP + ch;
 #pragma unroll 8
             for (uint32_t k = 0; k < here; k++) {
@@ -476,55 +623,60 @@ __global__ void __launch_bounds__(WARPS * 32, HDP == 64 ? 3 : 2) attend_kernel(A
               l[n] += sm_w[JOIN + k][h];
             }
           }
-          __syncthreads();
+          warps_sync();
         }
 #pragma unroll
         for (int n = 0; n < OWN; n++) {
           const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
-          if (h >= heads || (!FULL && ch >= a.hd)) continue;
+          if (h >= heads || ch >= a.hd) continue;
           const float f = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
           const float x[4] = {v[n].x * f, v[n].y * f, v[n].z * f, v[n].w * f};
 #pragma unroll
-          for (int e = 0; e < 4; e++) store_act(a.out, a.act, (size_t)r * a.out_stride + (size_t)(h0 + h) * a.hd + ch + e, x[e]);
+          for (int e = 0; e < 4; e++) store_act(a.out, a.act, (size_t)w.r * a.out_stride + (size_t)(h0 + h) * a.hd + ch + e, x[e]);
         }
         if (tid == 0) a.arrived[c0] = 0; // for the next call
       }
     }
-    __syncthreads(); // shared memory is free again
-    at += tile_end - tile;
-    tile = 0;
-    if (tile_end == tiles && ++which == per_row) {
-      row_at += tiles * per_row;
-      which = 0;
-      if (++r < a.rows) len = row_len(a, r, req), tiles = row_tiles(len);
-    }
+    warps_sync(); // shared memory is free again
+    next_segment<TP>(a, per_row, tile_end, w);
   }
 }
 
-constexpr uint32_t MAX_CTAS_PER_SM = 4;
+constexpr uint32_t MAX_CTAS_PER_SM = 3;
 
-template <typename C, int HDP, bool FULL, int TERMS>
-int launch_attend(FcDevice* dev, AttendArgs a) {
-  auto kern = attend_kernel<C, HDP, FULL, TERMS>;
-  static int resident[64]; // CTAs of an SM, by device
-  int& fit = resident[dev->ordinal & 63];
-  if (!fit) {
-    FC_CUDA(dev, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fit, kern, WARPS * 32, 0));
-    if (fit < 1 || fit > (int)MAX_CTAS_PER_SM) fit = fit < 1 ? 1 : MAX_CTAS_PER_SM;
+template <typename C>
+bool cache_map(CUtensorMap* map, const void* p, const FcPagedCache* c, uint32_t tile) {
+  const cuuint64_t es = sizeof(C), rows = (cuuint64_t)c->kv_heads * c->page;
+  const cuuint64_t dims[3] = {c->head_dim, rows, c->n_pages}, strides[2] = {c->head_dim * es, rows * c->head_dim * es};
+  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), c->page < tile ? c->page : tile, 1}, estr[3] = {1, 1, 1};
+  const CUtensorMapDataType type = std::is_same<C, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : std::is_same<C, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode_fn() && encode_fn()(map, type, 3, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename C, int HDP, int TERMS>
+int launch_attend(FcDevice* dev, const FcPagedCache* c, const AttendArgs& a) {
+  using S = Shape<C, HDP>;
+  auto kern = attend_kernel<C, HDP, TERMS>;
+  static OncePerDevice once;
+  if (once.first(dev->ordinal)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES);
+    if (e != cudaSuccess) once.again(dev->ordinal);
+    FC_CUDA(dev, e);
   }
-  const uint64_t most = (uint64_t)a.rows * a.kv_heads * a.blocks * (((((uint64_t)a.max_pages << a.page_shift) + TILE - 1) / TILE));
-  const uint64_t ctas = (uint64_t)dev->prop.multiProcessorCount * fit;
-  FC_LAUNCH(dev, "paged_attend", launch_on(dev, true, kern, dim3((unsigned)(most < ctas ? most : ctas)), dim3(WARPS * 32), 0, a));
+  CUtensorMap mk, mv;
+  if (!cache_map<C>(&mk, c->k, c, S::TP) || !cache_map<C>(&mv, c->v, c, S::TP))
+    return fc_fail(dev, FC_ERR_DEVICE, "no tensor map for a pool of %u pages of %u x %u x %u", c->n_pages, c->kv_heads, c->page, c->head_dim);
+  const uint64_t most = (uint64_t)a.rows * a.kv_heads * a.blocks * (((((uint64_t)a.max_pages << a.page_shift) + S::TP - 1) / S::TP));
+  const uint64_t ctas = (uint64_t)dev->prop.multiProcessorCount * S::CTAS;
+  FC_LAUNCH(dev, "paged_attend", launch_on(dev, true, kern, dim3((unsigned)(most < ctas ? most : ctas)), dim3(THREADS), S::BYTES, mk, mv, a));
   return FC_OK;
 }
 template <typename C, int TERMS>
-int launch_attend(FcDevice* dev, const AttendArgs& a) {
-  return a.hd == 64    ? launch_attend<C, 64, true, TERMS>(dev, a)
-         : a.hd < 64   ? launch_attend<C, 64, false, TERMS>(dev, a)
-         : a.hd == 128 ? launch_attend<C, 128, true, TERMS>(dev, a)
-         : a.hd < 128  ? launch_attend<C, 128, false, TERMS>(dev, a)
-         : a.hd == 256 ? launch_attend<C, 256, true, TERMS>(dev, a)
-                       : launch_attend<C, 256, false, TERMS>(dev, a);
+int launch_attend(FcDevice* dev, const FcPagedCache* c, const AttendArgs& a) {
+  return a.hd <= 64 ? launch_attend<C, 64, TERMS>(dev, c, a) : a.hd <= 128 ? launch_attend<C, 128, TERMS>(dev, c, a) : launch_attend<C, 256, TERMS>(dev, c, a);
 }
 
 // Partial results and arrival counters, for the handle's life: two parts per CTA that can be resident. The counters start at
@@ -546,6 +698,7 @@ int attend_scratch(FcDevice* dev, AttendArgs* a) {
     FC_CUDA(dev, cudaMemsetAsync(dev->attend.p, 0, words, dev->stream));
     dev->attend_clear = !stream_capturing(dev);
   }
+  a->err_flag = dev->d_flag;
   a->arrived = static_cast<uint32_t*>(dev->attend.p);
   a->parts = reinterpret_cast<float*>(static_cast<char*>(dev->attend.p) + words);
   return FC_OK;
@@ -572,7 +725,7 @@ FC_API int fc_paged_attend_dev(FcDevice* dev, const FcPagedCache* c, const void*
   if (!std::isfinite(scale)) return fc_fail(dev, FC_ERR_ARG, "the scale is not finite");
   if (!request && rows > c->requests) return fc_fail(dev, FC_ERR_RANGE, "%u rows in a table of %u requests", rows, c->requests);
   if (!rows) return FC_OK;
-  const uint64_t row_most = ((uint64_t)c->max_pages * c->page + TILE - 1) / TILE;
+  const uint64_t row_most = ((uint64_t)c->max_pages * c->page + 7) / 8;
   if ((uint64_t)rows * heads * row_most > 0xffffffffull) // (tiles are counted in 32 bits)
     return fc_fail(dev, FC_ERR_UNSUPPORTED, "%u rows of %u heads over page tables of %u x %u positions: more than one call holds", rows, heads,
                    c->max_pages, c->page);
@@ -583,8 +736,8 @@ FC_API int fc_paged_attend_dev(FcDevice* dev, const FcPagedCache* c, const void*
   a.rows = rows, a.group = heads / c->kv_heads, a.blocks = (a.group + ROWS8 - 1) / ROWS8, a.act = kind;
   a.scale = (scale == 0.0f ? 1.0f / sqrtf((float)c->head_dim) : scale) * 1.44269504088896340736f;
   FC_TRY(attend_scratch(dev, &a));
-  if (c->kind == FC_F32) return launch_attend<float, 2>(dev, a);
-  if (c->kind == FC_F16) return launch_attend<__half, 2>(dev, a);
+  if (c->kind == FC_F32) return launch_attend<float, 2>(dev, c, a);
+  if (c->kind == FC_F16) return launch_attend<__half, 2>(dev, c, a);
   // bf16 terms have 8 bits: two hold a 16-bit row, f32 rows take three
-  return kind == FC_F32 ? launch_attend<__nv_bfloat16, 3>(dev, a) : launch_attend<__nv_bfloat16, 2>(dev, a);
+  return kind == FC_F32 ? launch_attend<__nv_bfloat16, 3>(dev, c, a) : launch_attend<__nv_bfloat16, 2>(dev, c, a);
 }
