@@ -23,6 +23,11 @@ struct Workspace { // device scratch and its size
   size_t bytes = 0;
 };
 
+struct ServingScratch { // partial results of an operator and, first, the counters that join them
+  Workspace ws;
+  bool clear = false; // the counters have been zeroed (every call leaves them at zero)
+};
+
 struct FcDevice {
   int ordinal = 0;
   cudaStream_t stream = nullptr;
@@ -39,8 +44,7 @@ struct FcDevice {
   Workspace scratch;
   uint32_t weights = 0; // stand-alone weights alive
   cudaMemPool_t workspaces = nullptr;
-  Workspace attend;          // of the attention over a paged cache, from its first call on (paged_attend.cu)
-  bool attend_clear = false; // its counters have been zeroed
+  ServingScratch attend, logprobs; // of the operators of a paged cache, from their first call on
   int* d_flag = nullptr;   // device int for kernels that report a status
   int matvec_choice = 0;   // fc_debug_matvec_kernel: which kernel multiplies 1..8 rows (0: the library's rule)
   // per-kernel timing (off by default): one event pair per launch, summed by name on report

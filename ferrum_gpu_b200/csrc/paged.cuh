@@ -29,3 +29,6 @@ constexpr uint32_t PAGED_MAX_PAGE = 256, PAGED_MAX_HEAD_DIM = 256;
 // paged_plan.cu: the fields of a view that every entry point reads, and those of its k and v
 int paged_check_pages(FcDevice* dev, const FcPagedCache* c);
 int paged_check_pool(FcDevice* dev, const FcPagedCache* c);
+// An operator's scratch, `bytes` for the handle's life, of which the first `zero` start at zero. Allocated by the operator's
+// first call, under a stream capture too (no stream operation).
+int serving_scratch(FcDevice* dev, ServingScratch* s, size_t zero, size_t bytes, void** out);

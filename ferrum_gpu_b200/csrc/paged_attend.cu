@@ -683,24 +683,11 @@ int launch_attend(FcDevice* dev, const FcPagedCache* c, const AttendArgs& a) {
 // zero and every call leaves them there.
 int attend_scratch(FcDevice* dev, AttendArgs* a) {
   const size_t ctas = (size_t)dev->prop.multiProcessorCount * MAX_CTAS_PER_SM, words = (ctas * 4 + 255) / 256 * 256;
-  if (!dev->attend.p) {
-    const size_t bytes = words + ctas * 2 * part_floats(PAGED_MAX_HEAD_DIM) * 4;
-    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed; // (an allocation of its own, no stream operation: fine under a capture)
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    void* p = nullptr;
-    const cudaError_t e = stream_capturing(dev) ? cudaMalloc(&p, bytes) : device_malloc(dev, &p, bytes);
-    cudaThreadExchangeStreamCaptureMode(&mode);
-    FC_CUDA(dev, e);
-    dev->attend = Workspace{p, bytes};
-    dev->attend_clear = false;
-  }
-  if (!dev->attend_clear) { // (captured: a node of the graph, and the handle's own calls still have to do it once)
-    FC_CUDA(dev, cudaMemsetAsync(dev->attend.p, 0, words, dev->stream));
-    dev->attend_clear = !stream_capturing(dev);
-  }
+  void* p;
+  FC_TRY(serving_scratch(dev, &dev->attend, words, words + ctas * 2 * part_floats(PAGED_MAX_HEAD_DIM) * 4, &p));
   a->err_flag = dev->d_flag;
-  a->arrived = static_cast<uint32_t*>(dev->attend.p);
-  a->parts = reinterpret_cast<float*>(static_cast<char*>(dev->attend.p) + words);
+  a->arrived = static_cast<uint32_t*>(p);
+  a->parts = reinterpret_cast<float*>(static_cast<char*>(p) + words);
   return FC_OK;
 }
 

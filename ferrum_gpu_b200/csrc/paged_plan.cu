@@ -247,6 +247,26 @@ int plan_args(FcDevice* dev, const FcPagedCache* c, const int32_t* req, uint32_t
 
 } // namespace
 
+int serving_scratch(FcDevice* dev, ServingScratch* s, size_t zero, size_t bytes, void** out) {
+  const bool fresh = !s->ws.p;
+  if (fresh || !s->clear) {
+    const bool capturing = stream_capturing(dev);
+    if (fresh) {
+      cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      void* p = nullptr;
+      const cudaError_t e = capturing ? cudaMalloc(&p, bytes) : device_malloc(dev, &p, bytes);
+      cudaThreadExchangeStreamCaptureMode(&mode);
+      FC_CUDA(dev, e);
+      s->ws = Workspace{p, bytes};
+    }
+    FC_CUDA(dev, cudaMemsetAsync(s->ws.p, 0, zero, dev->stream)); // (captured: a node of the graph; the handle's own calls still do it once)
+    s->clear = !capturing;
+  }
+  *out = s->ws.p;
+  return FC_OK;
+}
+
 int paged_check_pages(FcDevice* dev, const FcPagedCache* c) {
   if (!c) return fc_fail(dev, FC_ERR_ARG, "the cache's view is NULL");
   if (c->page == 0 || c->page > PAGED_MAX_PAGE || (c->page & (c->page - 1)))
