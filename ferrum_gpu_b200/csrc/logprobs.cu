@@ -21,11 +21,10 @@
 namespace {
 
 constexpr uint32_t TOP_MAX = 32;
-constexpr int LP_THREADS = 256, LP_WARPS = LP_THREADS / 32;
-constexpr int LP_VECS = 8;          // 16-byte loads of a thread in flight
-constexpr uint32_t LP_GROUPS = 8;   // groups of a thread: their maxima are written down
-constexpr uint32_t LP_CTAS = 4;     // CTAs resident on an SM
-constexpr uint32_t LP_CAND = 1024;  // logits put in order by counting
+constexpr int LP_THREADS = 128, LP_WARPS = LP_THREADS / 32;
+constexpr uint32_t LP_GROUPS = 32;  // groups of a thread's logits in a row, over all its shares: their maxima are written down
+constexpr uint32_t LP_CTAS = 8;     // CTAs resident on an SM
+constexpr uint32_t LP_CAND = 512;   // logits put in order by counting
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
 struct Share { // of a row
@@ -36,14 +35,14 @@ struct Share { // of a row
 struct LogprobArgs {
   const void* logits;
   uint64_t stride;
-  uint32_t vocab, top, splits;
+  uint32_t vocab, top, splits, groups; // groups: of a share
   const int32_t* targets;
   float *logprob, *entropy;
   int32_t* rank;
   int32_t* top_index;
   float* top_logprob;
   Share* shares;      // [rows][splits]
-  float* maxima;      // [rows][splits][LP_GROUPS][LP_THREADS]
+  float* maxima;      // [rows][splits * groups][LP_THREADS]
   uint32_t* arrived;  // [rows]
 };
 
@@ -91,6 +90,50 @@ __device__ __forceinline__ void move_to(float m, Share& a) {
 template <typename T>
 struct Vec { // 16 bytes of logits
   static constexpr int E = 16 / sizeof(T);
+  static constexpr uint32_t STEP = 32 / E; // of them a thread has in flight: 32 logits (twice as many: more code than the instruction cache likes)
+  // all NaN or nothing: -inf
+  static __device__ __forceinline__ float high(const uint4& v) {
+    if constexpr (sizeof(T) == 4) {
+      return fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)), fmaxf(__uint_as_float(v.z), __uint_as_float(v.w)));
+    } else if constexpr (std::is_same<T, __half>::value) {
+      const __half2* h = reinterpret_cast<const __half2*>(&v);
+      const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(f.x, f.y);
+    } else {
+      const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+      const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+      return fmaxf(f.x, f.y);
+    }
+  }
+  // logits above thr; up to 128 per call (a half2 counts its halves)
+  template <uint32_t N>
+  static __device__ __forceinline__ uint32_t count(const uint4 (&v)[N], const T (&thr)[N]) {
+    if constexpr (sizeof(T) == 4) {
+      uint32_t n = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < N; i++)
+        n += (__uint_as_float(v[i].x) > thr[i]) + (__uint_as_float(v[i].y) > thr[i]) + (__uint_as_float(v[i].z) > thr[i]) + (__uint_as_float(v[i].w) > thr[i]);
+      return n;
+    } else if constexpr (std::is_same<T, __half>::value) {
+      __half2 n = __float2half2_rn(0.0f);
+#pragma unroll
+      for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) n = __hadd2(n, __hgt2(reinterpret_cast<const __half2*>(&v[i])[j], __half2half2(thr[i])));
+      return (uint32_t)(__low2float(n) + __high2float(n));
+    } else {
+      __nv_bfloat162 n = __float2bfloat162_rn(0.0f);
+#pragma unroll
+      for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) n = __hadd2(n, __hgt2(reinterpret_cast<const __nv_bfloat162*>(&v[i])[j], __bfloat162bfloat162(thr[i])));
+      return (uint32_t)(__low2float(n) + __high2float(n));
+    }
+  }
+  static __device__ __forceinline__ uint4 nothing() { // -inf everywhere
+    const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+    return make_uint4(w, w, w, w);
+  }
   static __device__ __forceinline__ void unpack(const uint4& v, float (&x)[E]) {
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -108,10 +151,35 @@ struct Vec { // 16 bytes of logits
 };
 
 // (exponentials below 2^-150 are 0, and so is their part of T: no 0 * inf)
+constexpr float LOWEST = -160.0f;
 __device__ __forceinline__ void add(float d, float& s, float& t) {
-  d = max_nan(d, -160.0f);
+  d = max_nan(d, LOWEST);
   const float e = ex2(d);
   s += e, t = fmaf(e, d, t);
+}
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// The next value below x (not NaN, not -inf); x - 0 and +0 alike.
+__device__ __forceinline__ uint32_t step_down(uint32_t bits, uint32_t sign) { return (bits & ~sign) == 0 ? sign | 1 : bits & sign ? bits + 1 : bits - 1; }
+__device__ __forceinline__ float next_below(float x) { return __uint_as_float(step_down(__float_as_uint(x), 0x80000000u)); }
+__device__ __forceinline__ __half next_below(__half x) { return __ushort_as_half((unsigned short)step_down(__half_as_ushort(x), 0x8000u)); }
+__device__ __forceinline__ __nv_bfloat16 next_below(__nv_bfloat16 x) {
+  return __ushort_as_bfloat16((unsigned short)step_down(__bfloat16_as_ushort(x), 0x8000u));
 }
 
 template <typename V, typename F>
@@ -119,6 +187,17 @@ __device__ __forceinline__ V warp_reduce(V v, F f) {
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
+}
+// three sums of the CTA's shares, all relative to one maximum
+__device__ __forceinline__ Share add_up(Share a, Share* sm) {
+  auto plus = [](auto x, auto y) { return x + y; };
+  a.s = warp_reduce(a.s, plus), a.t = warp_reduce(a.t, plus), a.above = warp_reduce(a.above, plus);
+  if ((threadIdx.x & 31) == 0) sm[threadIdx.x >> 5] = a;
+  __syncthreads();
+  a = sm[0];
+#pragma unroll
+  for (int w = 1; w < LP_WARPS; w++) a.s += sm[w].s, a.t += sm[w].t, a.above += sm[w].above;
+  return a;
 }
 // of the whole CTA; `sm`: a word per warp, free again after the call's second barrier
 template <typename V, typename F>
@@ -132,15 +211,15 @@ __device__ __forceinline__ V reduce(V v, V* sm, F f) {
   __syncthreads();
   return v;
 }
-// The warp's 32 keys in descending order over the lanes (bitonic); `from`: of a sequence that rises and falls only the last
-// rounds are needed.
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v, int from) {
+// The warp's 32 keys in descending order over the lanes (bitonic).
+__device__ __forceinline__ uint32_t sort_lanes(uint32_t v) {
   const uint32_t lane = threadIdx.x & 31;
-  for (int size = from; size <= 32; size <<= 1)
+#pragma unroll 1
+  for (int size = 2; size <= 32; size <<= 1)
+#pragma unroll 1
     for (int stride = size >> 1; stride; stride >>= 1) {
       const uint32_t other = __shfl_xor_sync(0xffffffffu, v, stride);
-      const bool low = (lane & stride) == 0, down = (lane & size) == 0 || size == 32;
-      v = low == down ? max(v, other) : min(v, other);
+      v = ((lane & stride) == 0) == ((lane & size) == 0) ? max(v, other) : min(v, other);
     }
   return v;
 }
@@ -164,90 +243,100 @@ struct Row {
 template <typename T>
 __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobArgs a) {
   constexpr int E = Vec<T>::E;
-  __shared__ float sm_f[LP_WARPS];
-  __shared__ uint32_t sm_u[LP_WARPS];
-  __shared__ float own_maxima[LP_GROUPS * LP_THREADS];
-  __shared__ uint32_t sm_sorted[LP_WARPS][32], sm_n, sm_ties, sm_last;
+  constexpr uint32_t VECS = Vec<T>::STEP, STEP = LP_THREADS * VECS;
+  __shared__ float sm_f[LP_WARPS], sm_ln;
+  __shared__ uint32_t sm_u[LP_WARPS], sm_n, sm_ties, sm_listed, sm_last;
+  __shared__ Share sm_share[LP_WARPS];
+  __shared__ float own_maxima[LP_GROUPS * LP_THREADS]; // of the row, in the end: a thread reads and writes its own column
+  __shared__ uint32_t sm_sets[32], listed[LP_CAND];
   __shared__ unsigned long long cand[LP_CAND];
   grid_wait();
   const uint32_t r = blockIdx.x / a.splits, split = blockIdx.x - r * a.splits, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Row<T> row(a, r);
   const int32_t target = a.targets ? a.targets[r] : -1;
   const bool has = (uint32_t)target < a.vocab;
-  const float xt = has ? to_f32(row.x[target]) : 0.0f;
-  // Logits before the target count where they are equal to it, those behind it where they are larger: larger than the next
-  // smaller value, and than it. A NaN target counts all that are no NaN; nothing else does.
-  const float behind = !has ? INFINITY : xt != xt ? -INFINITY : xt, before = !has ? INFINITY : xt != xt ? -INFINITY : xt == -INFINITY ? -INFINITY : nextafterf(xt, -INFINITY);
-  const bool floor_too = has && (xt != xt || xt == -INFINITY); // (nothing is smaller than -inf: compared with >= there)
-  auto ranks_before = [&](float x, uint32_t i) { return has && (xt != xt ? x == x : x > xt || (x == xt && i < (uint32_t)target)); };
+  const T raw_target = has ? row.x[target] : from_f32<T>(INFINITY);
+  const float xt = to_f32(raw_target);
+  // Logits before the target rank before it where they are not smaller, those behind it where they are larger: larger than the
+  // next value below it, and than it. (Nothing lies below -inf and nothing compares with NaN: counted in a sweep of their own.)
+  const bool sweep = has && !(xt > -INFINITY);
+  const T behind = sweep ? from_f32<T>(INFINITY) : raw_target, before = has && !sweep ? next_below(raw_target) : from_f32<T>(INFINITY);
 
-  // this CTA's share of the vectors, a thread's in steps of LP_VECS, `per` steps to a group
-  const uint32_t v0 = (uint32_t)((uint64_t)row.vecs * split / a.splits), v1 = (uint32_t)((uint64_t)row.vecs * (split + 1) / a.splits);
-  constexpr uint32_t STEP = LP_THREADS * LP_VECS;
-  const uint32_t steps = (v1 - v0 + STEP - 1) / STEP, per = (steps + LP_GROUPS - 1) / LP_GROUPS;
-  float* maxima = a.splits == 1 ? own_maxima : a.maxima + (size_t)blockIdx.x * (LP_GROUPS * LP_THREADS);
+  // this CTA's share of the vectors, a thread's in steps, `per` steps to a group
+  const uint32_t share = row.vecs / a.splits, extra = row.vecs - share * a.splits; // (the first `extra` shares take one more)
+  auto share_at = [&](uint32_t s) { return s * share + min(s, extra); };
+  const uint32_t v0 = share_at(split), v1 = share_at(split + 1);
+  const uint32_t per = max(1u, ((share + (extra ? 1 : 0) + STEP - 1) / STEP + a.groups - 1) / a.groups);
+  float* maxima = a.splits == 1 ? own_maxima : a.maxima + (size_t)blockIdx.x * a.groups * LP_THREADS;
   Share own{-INFINITY, 0.0f, 0.0f, 0u};
-  float group_max = -INFINITY;
-  uint32_t group = 0;
-  for (uint32_t st = 0; st < steps; st++) {
-    uint4 v[LP_VECS];
-    const uint32_t at = v0 + st * STEP + tid;
+  uint32_t at = v0 + tid;
+  for (uint32_t g = 0; g < a.groups; g++) {
+    float group_max = -INFINITY; // (of NaN or nothing: -inf, which reaches nothing that it should not)
+    for (uint32_t st = 0; st < per && at - tid < v1; st++, at += STEP) {
+      uint4 v[VECS];
 #pragma unroll
-    for (int i = 0; i < LP_VECS; i++)
-      if (at + i * LP_THREADS < v1) v[i] = __ldg(row.vec(at + i * LP_THREADS));
-    const int n = at < v1 ? min(LP_VECS, (int)((v1 - at + LP_THREADS - 1) / LP_THREADS)) : 0;
-    float high = -INFINITY;
+      for (uint32_t i = 0; i < VECS; i++) v[i] = at + i * LP_THREADS < v1 ? __ldg(row.vec(at + i * LP_THREADS)) : Vec<T>::nothing();
+      float high = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < LP_VECS; i++)
-      if (i < n) {
+      for (uint32_t i = 0; i < VECS; i++) high = fmaxf(high, Vec<T>::high(v[i]));
+      group_max = fmaxf(group_max, high);
+      if (high > own.m) move_to(high, own);
+      const Base base(own.m);
+      T thr[VECS]; // (the target's own vector: below)
+#pragma unroll
+      for (uint32_t i = 0; i < VECS; i++) thr[i] = row.head + (at + i * LP_THREADS) * E + E <= (uint32_t)target ? before : behind;
+      own.above += Vec<T>::count(v, thr);
+      if (base.big) { // (logits past 2^16: slowly, once more from memory)
+#pragma unroll 1
+        for (uint32_t i = 0; i < VECS * E; i++) {
+          const uint32_t vec = at + i / E * LP_THREADS;
+          if (vec >= v1) break;
+          add(base.of(to_f32(row.x[row.head + vec * E + i % E])), own.s, own.t);
+        }
+        continue;
+      }
+      const f32x2 scale = pack2(LOG2E, LOG2E), down = pack2(-base.l2, -base.l2);
+      f32x2 s = 0, t = 0;
+#pragma unroll
+      for (uint32_t i = 0; i < VECS; i++) {
+        if (at + i * LP_THREADS >= v1) break;
         float x[E];
         Vec<T>::unpack(v[i], x);
 #pragma unroll
-        for (int e = 0; e < E; e++) high = fmaxf(high, x[e]); // (a group of NaN: -inf, which reaches nothing that it should not)
-      }
-    group_max = fmaxf(group_max, high);
-    if (high > own.m) move_to(high, own);
-    const Base base(own.m);
-    auto sums = [&](auto big) {
-#pragma unroll
-      for (int i = 0; i < LP_VECS; i++)
-        if (i < n) {
-          float x[E];
-          Vec<T>::unpack(v[i], x);
-          const uint32_t first = row.head + (at + i * LP_THREADS) * E;
-          const float thr = first + E <= (uint32_t)target ? before : behind; // (the target's own vector: looked at below)
-#pragma unroll
-          for (int e = 0; e < E; e++) {
-            add(decltype(big)::value ? (x[e] - base.m) * LOG2E : fmaf(x[e], LOG2E, -base.l2), own.s, own.t);
-            own.above += x[e] > thr;
-          }
-          if (floor_too || (has && first <= (uint32_t)target && (uint32_t)target < first + E)) {
-#pragma unroll
-            for (int e = 0; e < E; e++) own.above += (uint32_t)ranks_before(x[e], first + e) - (uint32_t)(x[e] > thr);
-          }
+        for (int e = 0; e < E; e += 2) {
+          float d0, d1;
+          unpack2(fma2(pack2(x[e], x[e + 1]), scale, down), d0, d1);
+          d0 = max_nan(d0, LOWEST), d1 = max_nan(d1, LOWEST);
+          const f32x2 p = pack2(ex2(d0), ex2(d1));
+          s = add2(s, p), t = fma2(p, pack2(d0, d1), t);
         }
-    };
-    if (base.big) sums(std::true_type());
-    else sums(std::false_type());
-    if (a.top && ((st + 1) % per == 0 || st + 1 == steps)) {
-      maxima[group++ * LP_THREADS + tid] = group_max;
-      group_max = -INFINITY;
+      }
+      float s0, s1, t0, t1;
+      unpack2(s, s0, s1), unpack2(t, t0, t1);
+      own.s += s0 + s1, own.t += t0 + t1;
     }
+    if (a.top) maxima[g * LP_THREADS + tid] = group_max;
   }
   if (split == 0 && tid < row.rest) {
     const uint32_t i = row.rest_at(tid);
     const float x = to_f32(row.x[i]);
     if (x > own.m) move_to(x, own);
     add(Base(own.m).of(x), own.s, own.t);
-    own.above += ranks_before(x, i);
+    own.above += x > to_f32(i < (uint32_t)target ? before : behind);
   }
+  if (split == 0 && has && !sweep && tid == 0 && (uint32_t)target >= row.head && (uint32_t)target < row.head + row.vecs * E) {
+    // (the target's own vector was counted as if it lay behind the target)
+    for (uint32_t i = row.head + ((uint32_t)target - row.head) / E * E; i < (uint32_t)target; i++) own.above += to_f32(row.x[i]) == xt;
+  }
+  if (sweep)
+    for (uint32_t i = split * LP_THREADS + tid; i < a.vocab; i += a.splits * LP_THREADS) {
+      const float x = to_f32(row.x[i]);
+      own.above += xt != xt ? x == x : x > xt || (x == xt && i < (uint32_t)target);
+    }
   // the share
   auto larger = [](float x, float y) { return fmaxf(x, y); };
-  auto plus = [](auto x, auto y) { return x + y; };
-  const float m = reduce(own.m, sm_f, larger);
-  move_to(m, own);
-  Share all{m, reduce(own.s, sm_f, plus), reduce(own.t, sm_f, plus), reduce(own.above, sm_u, plus)};
-  uint32_t groups = (steps + max(per, 1u) - 1) / max(per, 1u);
+  move_to(reduce(own.m, sm_f, larger), own);
+  Share all = add_up(own, sm_share);
   if (a.splits > 1) {
     if (tid == 0) a.shares[blockIdx.x] = all;
     __threadfence();
@@ -268,59 +357,59 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     }
     const float top = reduce(mine.m, sm_f, larger);
     move_to(top, mine);
-    all = Share{top, reduce(mine.s, sm_f, plus), reduce(mine.t, sm_f, plus), reduce(mine.above, sm_u, plus)};
+    all = add_up(mine, sm_share); // (the barriers since the first use of sm_share lie behind everyone's reads)
   }
-  const Base base(all.m);
-  const float log_s = all.s == 0.0f ? 0.0f : log2f(all.s);
-  // ln of the sum relative to the maximum itself: less what rounding m log2 e left out
-  const float ln_s = LN2 * (log_s - base.left);
-  auto logprob_of = [&](float x) { return x - base.m - ln_s; };
+  const float top_logit = all.m == -INFINITY ? 0.0f : all.m;
   if (tid == 0) {
-    if (a.logprob) a.logprob[r] = has ? logprob_of(xt) : __int_as_float(0x7fffffff);
+    // ln of the sum relative to the maximum itself: less what rounding m log2 e left out
+    const float log_s = all.s == 0.0f ? 0.0f : log2f(all.s);
+    sm_ln = LN2 * (log_s - Base(all.m).left);
+    if (a.logprob) a.logprob[r] = has ? xt - top_logit - sm_ln : __int_as_float(0x7fffffff);
     if (a.entropy) a.entropy[r] = all.s == 0.0f ? 0.0f : LN2 * (log_s - all.t / all.s);
     if (a.rank) a.rank[r] = has ? (int32_t)all.above : -1;
+    sm_n = sm_ties = sm_listed = 0;
   }
   if (!a.top) return;
+  __syncthreads();
 
   // ---- the alternatives ----
   auto put = [&](uint32_t k, unsigned long long key) { // key 0: there is none
     const float x = value_of((uint32_t)(key >> 32));
     if (a.top_index) a.top_index[(size_t)r * a.top + k] = key ? (int32_t)(0xffffffffu - (uint32_t)key) : -1;
-    if (a.top_logprob) a.top_logprob[(size_t)r * a.top + k] = key ? logprob_of(x) : -INFINITY;
+    if (a.top_logprob) a.top_logprob[(size_t)r * a.top + k] = key ? x - top_logit - sm_ln : -INFINITY;
   };
   auto key_of = [](uint32_t order, uint32_t i) { return (unsigned long long)order << 32 | (0xffffffffu - i); };
-  // the shares' maxima: group g of thread t of share s covers steps g per .. of that share
-  const float* row_maxima = a.splits == 1 ? own_maxima : a.maxima + (size_t)r * a.splits * (LP_GROUPS * LP_THREADS);
-  auto share_groups = [&](uint32_t s, uint32_t& first, uint32_t& last, uint32_t& per) {
-    first = (uint32_t)((uint64_t)row.vecs * s / a.splits), last = (uint32_t)((uint64_t)row.vecs * (s + 1) / a.splits);
-    const uint32_t steps = (last - first + STEP - 1) / STEP;
-    per = (steps + LP_GROUPS - 1) / LP_GROUPS;
-    return per ? (steps + per - 1) / per : 0u;
-  };
-  __syncthreads(); // (own_maxima)
-  uint32_t best = 0;
-  for (uint32_t s = 0; s < a.splits; s++) {
-    uint32_t first, last, per_s;
-    const uint32_t n = share_groups(s, first, last, per_s);
-    for (uint32_t g = 0; g < n; g++) {
-      const float* p = row_maxima + (size_t)(s * LP_GROUPS + g) * LP_THREADS + tid;
-      best = max(best, order_of(a.splits == 1 ? *p : __ldcg(p)));
-    }
-  }
-  // the k-th largest of the threads' maxima: sorted per warp, then the larger halves of pairs of warps
-  uint32_t sorted = sort_lanes(best, 2);
-  sm_sorted[warp][lane] = sorted;
-  if (tid == 0) sm_n = 0, sm_ties = 0;
-  __syncthreads();
+  // This thread's group maxima, of all shares. The CTA's threads fall into 32 sets of 4: the k-th largest of the sets' maxima
+  // bounds the k-th largest logit (about k further logits lie above it; 130 for k = 32).
+  const uint32_t all_groups = a.splits * a.groups;
+  const float* row_maxima = a.maxima + (size_t)r * all_groups * LP_THREADS;
+  if (a.splits > 1)
+#pragma unroll 8
+    for (uint32_t i = 0; i < all_groups; i++) own_maxima[i * LP_THREADS + tid] = __ldcg(row_maxima + i * LP_THREADS + tid);
+  auto maximum = [&](uint32_t i) { return order_of(own_maxima[i * LP_THREADS + tid]); };
+  uint32_t bound = order_of(all.m); // one alternative: the maximum itself
+  if (a.top > 1) {
+    uint32_t best = 0;
+#pragma unroll 4
+    for (uint32_t i = 0; i < all_groups; i++) best = max(best, maximum(i));
 #pragma unroll
-  for (int half = LP_WARPS / 2; half; half >>= 1) {
-    if (warp < half) {
-      sorted = sort_lanes(max(sorted, sm_sorted[warp + half][31 - lane]), 32);
-      sm_sorted[warp][lane] = sorted;
+    for (int o = 1; o < LP_THREADS / 32; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
+    if (lane % (LP_THREADS / 32) == 0) sm_sets[tid / (LP_THREADS / 32)] = best;
+    __syncthreads();
+    bound = __shfl_sync(0xffffffffu, sort_lanes(sm_sets[lane]), a.top - 1);
+  }
+  // a share's groups all have as many steps; a group is listed as (share's group) * LP_THREADS + thread
+  auto list = [&](bool equal_too) {
+#pragma unroll 4
+    for (uint32_t i = 0; i < all_groups; i++) {
+      const uint32_t o = maximum(i);
+      if (o > bound || (o == bound && equal_too)) {
+        const uint32_t p = atomicAdd(&sm_listed, 1u);
+        if (p < LP_CAND) listed[p] = i * LP_THREADS + tid;
+      }
     }
     __syncthreads();
-  }
-  const uint32_t bound = sm_sorted[0][a.top - 1];
+  };
   // The logits above the bound, from the front of the list, and those equal to it, from its end.
   auto offer = [&](float x, uint32_t i, bool equal_too) {
     const uint32_t o = order_of(x);
@@ -329,47 +418,45 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     if (p < LP_CAND) cand[o > bound ? p : LP_CAND - 1 - p] = key_of(o, i);
   };
   auto gather = [&](bool equal_too) {
-    for (uint32_t s = 0; s < a.splits; s++) {
-      uint32_t first, last, per_s;
-      const uint32_t n = share_groups(s, first, last, per_s);
-      for (uint32_t g = 0; g < n; g++) {
-        const float* p = row_maxima + (size_t)(s * LP_GROUPS + g) * LP_THREADS + tid;
-        const uint32_t o = order_of(a.splits == 1 ? *p : __ldcg(p));
-        // a warp reads its groups that reach the bound one after another, a vector per lane
-        for (uint32_t reach = __ballot_sync(0xffffffffu, o > bound || (o == bound && equal_too)); reach; reach &= reach - 1) {
-          if (*(volatile uint32_t*)&sm_n + *(volatile uint32_t*)&sm_ties > LP_CAND) break; // (the list runs over: no use)
-          const uint32_t begin = first + g * per_s * STEP + warp * 32 + __ffs(reach) - 1;
-          for (uint32_t i = lane; i < per_s * LP_VECS; i += 32) {
-            const uint32_t at = begin + i * LP_THREADS;
-            if (at >= last) break;
-            float x[E];
-            Vec<T>::unpack(__ldg(row.vec(at)), x);
+    list(equal_too);
+    if (sm_listed <= LP_CAND) {
+      const uint32_t vecs = per * VECS, total = sm_listed * vecs;
+#pragma unroll 1
+      for (uint32_t j = tid; j < total; j += LP_THREADS) {
+        const uint32_t entry = listed[j / vecs], i = entry / LP_THREADS, s = i / a.groups, g = i - s * a.groups;
+        const uint32_t at = share_at(s) + (g * per * VECS + j % vecs) * LP_THREADS + entry % LP_THREADS;
+        if (at >= share_at(s + 1)) continue;
+        const uint4 v = __ldg(row.vec(at));
+        if (order_of(Vec<T>::high(v)) < bound) continue;
+        float x[E];
+        Vec<T>::unpack(v, x);
 #pragma unroll
-            for (int e = 0; e < E; e++) offer(x[e], row.head + at * E + e, equal_too);
-          }
-          __syncwarp();
-        }
+        for (int e = 0; e < E; e++) offer(x[e], row.head + at * E + e, equal_too);
       }
     }
     if (tid < row.rest) offer(to_f32(row.x[row.rest_at(tid)]), row.rest_at(tid), equal_too);
     __syncthreads();
-  };
-  gather(true);
-  const bool over = sm_n + sm_ties > LP_CAND;
-  __syncthreads();
-  if (over) { // many equal ones, as a rule: those above the bound alone
-    if (tid == 0) sm_n = 0, sm_ties = 0;
+    const bool fits = sm_listed <= LP_CAND && sm_n + sm_ties <= LP_CAND;
     __syncthreads();
-    gather(false);
+    return fits;
+  };
+  const bool over = bound == order_of(-INFINITY) || !gather(true); // (forbidden tokens are many at once)
+  bool fits = !over;
+  if (over) { // many equal ones, as a rule: those above the bound alone
+    if (tid == 0) sm_n = sm_ties = sm_listed = 0;
+    __syncthreads();
+    fits = gather(false);
   }
   const uint32_t above = sm_n, n = above + sm_ties;
-  if (n <= LP_CAND) {
+  if (fits) {
     // a candidate's place is the number of larger ones
     for (uint32_t i = tid; i < n; i += LP_THREADS) {
       const unsigned long long key = cand[i < above ? i : LP_CAND - 1 - (i - above)];
       uint32_t place = 0;
+#pragma unroll 4
       for (uint32_t j = 0; j < above; j++) place += cand[j] > key;
       if (i >= above)
+#pragma unroll 1
         for (uint32_t j = above; j < n; j++) place += cand[LP_CAND - 1 - (j - above)] > key;
       if (place < a.top) put(place, key);
     }
@@ -423,15 +510,16 @@ FC_API int fc_logprobs_dev(FcDevice* dev, const void* logits, int kind, uint32_t
   if (rows && !aligned_to(logits, paged_bytes(kind))) return fc_fail(dev, FC_ERR_ARG, "logits must be aligned to their elements");
   if (rows > (1u << 30)) return fc_fail(dev, FC_ERR_SHAPE, "%u rows", rows);
   if (!rows) return FC_OK;
-  LogprobArgs a{logits, stride, vocab, top_index || top_logprob ? top : 0u, 1u, targets, logprob, entropy, rank, top_index, top_logprob, nullptr, nullptr, nullptr};
+  LogprobArgs a{logits, stride, vocab, top_index || top_logprob ? top : 0u, 1u, 8u, targets, logprob, entropy, rank, top_index, top_logprob, nullptr, nullptr, nullptr};
   // shares of a row: as many as there are SMs' CTAs left for it, each of whole steps
   const uint32_t ctas = (uint32_t)dev->prop.multiProcessorCount * LP_CTAS;
-  const uint64_t vecs = (uint64_t)vocab * paged_bytes(kind) / 16, steps = (vecs + LP_THREADS * LP_VECS - 1) / (LP_THREADS * LP_VECS);
-  if (rows < ctas && steps > 1) a.splits = (uint32_t)(steps < ctas / rows ? steps : ctas / rows);
+  const uint64_t steps = ((uint64_t)vocab + LP_THREADS * 32 - 1) / (LP_THREADS * 32);
+  if (rows < ctas && steps > 1) a.splits = (uint32_t)min(min(steps, (uint64_t)(ctas / rows)), (uint64_t)LP_GROUPS);
   if (a.splits > 1) {
+    a.groups = min(8u, LP_GROUPS / a.splits);
     const size_t words = ((size_t)ctas * 4 + 255) / 256 * 256, shares = ((size_t)ctas * sizeof(Share) + 255) / 256 * 256;
     void* p;
-    FC_TRY(serving_scratch(dev, &dev->logprobs, words, words + shares + (size_t)ctas * LP_GROUPS * LP_THREADS * 4, &p));
+    FC_TRY(serving_scratch(dev, &dev->logprobs, words, words + shares + (size_t)ctas * 8 * LP_THREADS * 4, &p));
     a.arrived = static_cast<uint32_t*>(p);
     a.shares = reinterpret_cast<Share*>(static_cast<char*>(p) + words);
     a.maxima = reinterpret_cast<float*>(static_cast<char*>(p) + words + shares);
