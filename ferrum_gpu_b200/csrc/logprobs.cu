@@ -23,7 +23,7 @@ namespace {
 constexpr uint32_t TOP_MAX = 32;
 constexpr int LP_THREADS = 128, LP_WARPS = LP_THREADS / 32;
 constexpr uint32_t LP_GROUPS = 32;  // groups of a thread's logits in a row, over all its shares: their maxima are written down
-constexpr uint32_t LP_CTAS = 8;     // CTAs resident on an SM
+constexpr uint32_t LP_CTAS = 6;     // CTAs resident on an SM
 constexpr uint32_t LP_CAND = 512;   // logits put in order by counting
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
 
@@ -90,7 +90,7 @@ __device__ __forceinline__ void move_to(float m, Share& a) {
 template <typename T>
 struct Vec { // 16 bytes of logits
   static constexpr int E = 16 / sizeof(T);
-  static constexpr uint32_t STEP = 32 / E; // of them a thread has in flight: 32 logits (twice as many: more code than the instruction cache likes)
+  static constexpr uint32_t STEP = 4; // of them a thread works on, four more in flight
   // all NaN or nothing: -inf
   static __device__ __forceinline__ float high(const uint4& v) {
     if constexpr (sizeof(T) == 4) {
@@ -211,19 +211,6 @@ __device__ __forceinline__ V reduce(V v, V* sm, F f) {
   __syncthreads();
   return v;
 }
-// The warp's 32 keys in descending order over the lanes (bitonic).
-__device__ __forceinline__ uint32_t sort_lanes(uint32_t v) {
-  const uint32_t lane = threadIdx.x & 31;
-#pragma unroll 1
-  for (int size = 2; size <= 32; size <<= 1)
-#pragma unroll 1
-    for (int stride = size >> 1; stride; stride >>= 1) {
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, v, stride);
-      v = ((lane & stride) == 0) == ((lane & size) == 0) ? max(v, other) : min(v, other);
-    }
-  return v;
-}
-
 // Where a row's logits lie: vectors from the first 16-byte boundary on, and the few before and behind them.
 template <typename T>
 struct Row {
@@ -253,15 +240,6 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   grid_wait();
   const uint32_t r = blockIdx.x / a.splits, split = blockIdx.x - r * a.splits, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Row<T> row(a, r);
-  const int32_t target = a.targets ? a.targets[r] : -1;
-  const bool has = (uint32_t)target < a.vocab;
-  const T raw_target = has ? row.x[target] : from_f32<T>(INFINITY);
-  const float xt = to_f32(raw_target);
-  // Logits before the target rank before it where they are not smaller, those behind it where they are larger: larger than the
-  // next value below it, and than it. (Nothing lies below -inf and nothing compares with NaN: counted in a sweep of their own.)
-  const bool sweep = has && !(xt > -INFINITY);
-  const T behind = sweep ? from_f32<T>(INFINITY) : raw_target, before = has && !sweep ? next_below(raw_target) : from_f32<T>(INFINITY);
-
   // this CTA's share of the vectors, a thread's in steps, `per` steps to a group
   const uint32_t share = row.vecs / a.splits, extra = row.vecs - share * a.splits; // (the first `extra` shares take one more)
   auto share_at = [&](uint32_t s) { return s * share + min(s, extra); };
@@ -270,12 +248,27 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   float* maxima = a.splits == 1 ? own_maxima : a.maxima + (size_t)blockIdx.x * a.groups * LP_THREADS;
   Share own{-INFINITY, 0.0f, 0.0f, 0u};
   uint32_t at = v0 + tid;
+  uint4 v[VECS], next[VECS];
+  auto load = [&](uint4 (&v)[VECS], uint32_t at) {
+#pragma unroll
+    for (uint32_t i = 0; i < VECS; i++) v[i] = at + i * LP_THREADS < v1 ? __ldg(row.vec(at + i * LP_THREADS)) : Vec<T>::nothing();
+  };
+  load(v, at);
+  // (the target's logit is asked for behind the first vectors: its address is a load away itself)
+  const int32_t target = a.targets ? a.targets[r] : -1;
+  const bool has = (uint32_t)target < a.vocab;
+  const T raw_target = has ? row.x[target] : from_f32<T>(INFINITY);
+  const float xt = to_f32(raw_target);
+  // Logits before the target rank before it where they are not smaller, those behind it where they are larger: larger than the
+  // next value below it, and than it. (Nothing lies below -inf and nothing compares with NaN: counted in a sweep of their own.)
+  const bool sweep = has && !(xt > -INFINITY);
+  const T behind = sweep ? from_f32<T>(INFINITY) : raw_target, before = has && !sweep ? next_below(raw_target) : from_f32<T>(INFINITY);
   for (uint32_t g = 0; g < a.groups; g++) {
     float group_max = -INFINITY; // (of NaN or nothing: -inf, which reaches nothing that it should not)
-    for (uint32_t st = 0; st < per && at - tid < v1; st++, at += STEP) {
-      uint4 v[VECS];
-#pragma unroll
-      for (uint32_t i = 0; i < VECS; i++) v[i] = at + i * LP_THREADS < v1 ? __ldg(row.vec(at + i * LP_THREADS)) : Vec<T>::nothing();
+    for (uint32_t st = 0; st < per && at - tid < v1; st++) {
+      const uint32_t now = at;
+      at += STEP;
+      load(next, at);
       float high = -INFINITY;
 #pragma unroll
       for (uint32_t i = 0; i < VECS; i++) high = fmaxf(high, Vec<T>::high(v[i]));
@@ -284,36 +277,38 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
       const Base base(own.m);
       T thr[VECS]; // (the target's own vector: below)
 #pragma unroll
-      for (uint32_t i = 0; i < VECS; i++) thr[i] = row.head + (at + i * LP_THREADS) * E + E <= (uint32_t)target ? before : behind;
+      for (uint32_t i = 0; i < VECS; i++) thr[i] = row.head + (now + i * LP_THREADS) * E + E <= (uint32_t)target ? before : behind;
       own.above += Vec<T>::count(v, thr);
       if (base.big) { // (logits past 2^16: slowly, once more from memory)
 #pragma unroll 1
         for (uint32_t i = 0; i < VECS * E; i++) {
-          const uint32_t vec = at + i / E * LP_THREADS;
+          const uint32_t vec = now + i / E * LP_THREADS;
           if (vec >= v1) break;
           add(base.of(to_f32(row.x[row.head + vec * E + i % E])), own.s, own.t);
         }
-        continue;
-      }
-      const f32x2 scale = pack2(LOG2E, LOG2E), down = pack2(-base.l2, -base.l2);
-      f32x2 s = 0, t = 0;
+      } else {
+        const f32x2 scale = pack2(LOG2E, LOG2E), down = pack2(-base.l2, -base.l2);
+        f32x2 s = 0, t = 0;
 #pragma unroll
-      for (uint32_t i = 0; i < VECS; i++) {
-        if (at + i * LP_THREADS >= v1) break;
-        float x[E];
-        Vec<T>::unpack(v[i], x);
+        for (uint32_t i = 0; i < VECS; i++) {
+          if (now + i * LP_THREADS >= v1) break;
+          float x[E];
+          Vec<T>::unpack(v[i], x);
 #pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          float d0, d1;
-          unpack2(fma2(pack2(x[e], x[e + 1]), scale, down), d0, d1);
-          d0 = max_nan(d0, LOWEST), d1 = max_nan(d1, LOWEST);
-          const f32x2 p = pack2(ex2(d0), ex2(d1));
-          s = add2(s, p), t = fma2(p, pack2(d0, d1), t);
+          for (int e = 0; e < E; e += 2) {
+            float d0, d1;
+            unpack2(fma2(pack2(x[e], x[e + 1]), scale, down), d0, d1);
+            d0 = max_nan(d0, LOWEST), d1 = max_nan(d1, LOWEST);
+            const f32x2 p = pack2(ex2(d0), ex2(d1));
+            s = add2(s, p), t = fma2(p, pack2(d0, d1), t);
+          }
         }
+        float s0, s1, t0, t1;
+        unpack2(s, s0, s1), unpack2(t, t0, t1);
+        own.s += s0 + s1, own.t += t0 + t1;
       }
-      float s0, s1, t0, t1;
-      unpack2(s, s0, s1), unpack2(t, t0, t1);
-      own.s += s0 + s1, own.t += t0 + t1;
+#pragma unroll
+      for (uint32_t i = 0; i < VECS; i++) v[i] = next[i];
     }
     if (a.top) maxima[g * LP_THREADS + tid] = group_max;
   }
@@ -339,13 +334,20 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   Share all = add_up(own, sm_share);
   if (a.splits > 1) {
     if (tid == 0) a.shares[blockIdx.x] = all;
-    __threadfence();
     __syncthreads();
-    if (tid == 0) sm_last = atomicAdd(&a.arrived[r], 1u) == a.splits - 1;
+    if (tid == 0) { // (the barriers carry the fences' order to the CTA's other threads)
+      __threadfence();
+      sm_last = atomicAdd(&a.arrived[r], 1u) == a.splits - 1;
+      __threadfence();
+    }
     __syncthreads();
     if (!sm_last) return;
-    __threadfence();
     if (tid == 0) a.arrived[r] = 0; // for the next call
+    if (a.top) {
+      const float* row_maxima = a.maxima + (size_t)r * (a.splits * a.groups) * LP_THREADS + tid;
+#pragma unroll 8
+      for (uint32_t i = 0; i < a.splits * a.groups; i++) own_maxima[i * LP_THREADS + tid] = __ldcg(row_maxima + i * LP_THREADS);
+    }
     const Share* shares = a.shares + (size_t)r * a.splits;
     Share mine{-INFINITY, 0.0f, 0.0f, 0u};
     for (uint32_t i = tid; i < a.splits; i += LP_THREADS) {
@@ -382,10 +384,6 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   // This thread's group maxima, of all shares. The CTA's threads fall into 32 sets of 4: the k-th largest of the sets' maxima
   // bounds the k-th largest logit (about k further logits lie above it; 130 for k = 32).
   const uint32_t all_groups = a.splits * a.groups;
-  const float* row_maxima = a.maxima + (size_t)r * all_groups * LP_THREADS;
-  if (a.splits > 1)
-#pragma unroll 8
-    for (uint32_t i = 0; i < all_groups; i++) own_maxima[i * LP_THREADS + tid] = __ldcg(row_maxima + i * LP_THREADS + tid);
   auto maximum = [&](uint32_t i) { return order_of(own_maxima[i * LP_THREADS + tid]); };
   uint32_t bound = order_of(all.m); // one alternative: the maximum itself
   if (a.top > 1) {
@@ -396,7 +394,11 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     for (int o = 1; o < LP_THREADS / 32; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
     if (lane % (LP_THREADS / 32) == 0) sm_sets[tid / (LP_THREADS / 32)] = best;
     __syncthreads();
-    bound = __shfl_sync(0xffffffffu, sort_lanes(sm_sets[lane]), a.top - 1);
+    const uint32_t mine = sm_sets[lane];
+    uint32_t place = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < 32; j++) place += sm_sets[j] > mine || (sm_sets[j] == mine && j < lane);
+    bound = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, place == a.top - 1)) - 1);
   }
   // a share's groups all have as many steps; a group is listed as (share's group) * LP_THREADS + thread
   auto list = [&](bool equal_too) {
@@ -421,7 +423,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     list(equal_too);
     if (sm_listed <= LP_CAND) {
       const uint32_t vecs = per * VECS, total = sm_listed * vecs;
-#pragma unroll 1
+#pragma unroll 2
       for (uint32_t j = tid; j < total; j += LP_THREADS) {
         const uint32_t entry = listed[j / vecs], i = entry / LP_THREADS, s = i / a.groups, g = i - s * a.groups;
         const uint32_t at = share_at(s) + (g * per * VECS + j % vecs) * LP_THREADS + entry % LP_THREADS;
@@ -513,7 +515,7 @@ FC_API int fc_logprobs_dev(FcDevice* dev, const void* logits, int kind, uint32_t
   LogprobArgs a{logits, stride, vocab, top_index || top_logprob ? top : 0u, 1u, 8u, targets, logprob, entropy, rank, top_index, top_logprob, nullptr, nullptr, nullptr};
   // shares of a row: as many as there are SMs' CTAs left for it, each of whole steps
   const uint32_t ctas = (uint32_t)dev->prop.multiProcessorCount * LP_CTAS;
-  const uint64_t steps = ((uint64_t)vocab + LP_THREADS * 32 - 1) / (LP_THREADS * 32);
+  const uint64_t steps = ((uint64_t)vocab * paged_bytes(kind) + LP_THREADS * 64 - 1) / (LP_THREADS * 64);
   if (rows < ctas && steps > 1) a.splits = (uint32_t)min(min(steps, (uint64_t)(ctas / rows)), (uint64_t)LP_GROUPS);
   if (a.splits > 1) {
     a.groups = min(8u, LP_GROUPS / a.splits);

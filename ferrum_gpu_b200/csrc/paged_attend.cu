@@ -576,14 +576,16 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
       };
       const uint32_t c0 = owner_of(first_tile), c1 = owner_of(first_tile + w.tiles - 1);
-      if (warp == 0) {
-        __threadfence();
+      if (warp == 0) { // (the part is this warp's own; the barriers carry the fences' order to the others)
         __syncwarp();
-        if (lane == 0) sm_last = atomicAdd(&a.arrived[c0], 1u) == c1 - c0;
+        if (lane == 0) {
+          __threadfence();
+          sm_last = atomicAdd(&a.arrived[c0], 1u) == c1 - c0;
+          __threadfence();
+        }
       }
       warps_sync();
       if (sm_last) {
-        __threadfence();
         // Each warp finds two heads' maxima over the parts; then, JOIN parts at a time, their weights go to shared memory and
         // every thread adds its channels' values, all loads of a turn in flight together.
         float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(shared);
