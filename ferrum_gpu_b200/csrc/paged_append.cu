@@ -5,15 +5,17 @@
 // whatever the rows' and the cache's type, rounded once when it is stored. The tables come with the call
 // (fc_rope_tables): angles of long contexts need 64 bits, the rotation does not.
 //
-// What bounds it is bytes: every row read and written once. A row is cut into items of up to N elements a load (16 bytes of a
-// 16-bit row): a run of N pairs of a head - one piece for neighbouring pairs, two for the half layout -, or N channels that are
-// only copied. Items of all rows are one line, so that small heads and few rows fill warps too; a thread has the loads of
-// two items in flight. The tables' rows are shared by all heads and come from L1 / L2.
+// What bounds it is bytes: every row read and written once. A row is cut into pieces of N elements (16 bytes of a 16-bit
+// row): a run of N pairs of a head - one piece for neighbouring pairs, two for the half layout -, or N channels that are only
+// copied. A thread takes the same piece of H heads, so that slot, position and the tables' values are fetched once for
+// them, and has the loads of all of them in flight; the pieces of all rows are one line, so that small heads and few rows
+// fill warps too. Calls of few rows, where latency counts, take one head a thread.
 #include <algorithm>
 #include <cmath>
 #include <vector>
 
 #include "paged.cuh"
+#include "tc_ptx.cuh"
 
 namespace {
 
@@ -37,11 +39,12 @@ struct AppendArgs {
   uint64_t stride, q_stride, slots;
   uint32_t rows, heads, kv_heads, hd, half, positions, page_shift;
   bool neox;
-  uint32_t turned;               // items of a head that are rotated
-  Div items, per_head, per_v;    // items of a row, of a q or k head, of a v head
+  int* err_flag;
+  uint32_t turned, turned_blocks; // pieces of a q or k head that are rotated; blocks of H heads that are q or k
+  Div items, per_head, per_v;     // items of a row, pieces of a q or k head, of a v head
 };
 
-constexpr int APPEND_THREADS = 256, IN_FLIGHT = 2;
+constexpr int APPEND_THREADS = 256;
 
 // N elements side by side, one or two accesses of up to 16 bytes
 template <typename T, int N>
@@ -93,83 +96,246 @@ __device__ __forceinline__ void store_run(T* p, const float (&x)[N]) {
   }
 }
 
-// N: elements of an item's piece; 1 also takes pairs that no wider piece meets, and rows aligned to nothing but elements
-template <typename T, typename C, int N>
+// N: elements of a piece (1 also takes pairs that no wider piece meets, and rows aligned to nothing but elements); H: heads
+// of an item
+template <typename T, typename C, int N, int H>
 __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendArgs a) {
   grid_wait();
   const uint32_t all = a.rows * a.items.d, threads = gridDim.x * APPEND_THREADS;
-  for (uint32_t first = blockIdx.x * APPEND_THREADS + threadIdx.x; first < all; first += threads * IN_FLIGHT) {
-    float x[IN_FLIGHT][N], y[IN_FLIGHT][N];
-    uint32_t row[IN_FLIGHT], head[IN_FLIGHT], ch[IN_FLIGHT]; // ch: the first piece's first channel; the second's lies `apart` behind
-    bool turn[IN_FLIGHT];
-    int32_t pos[IN_FLIGHT];
-    int64_t slot[IN_FLIGHT];
-    const uint32_t apart = a.neox ? a.half : 1u;
-#pragma unroll
-    for (int i = 0; i < IN_FLIGHT; i++) {
-      const uint32_t id = first + i * threads;
-      if (id >= all) break;
-      row[i] = a.items.of(id);
-      uint32_t it = id - row[i] * a.items.d;
-      const uint32_t rotating = (a.heads + a.kv_heads) * a.per_head.d;
-      if (it < rotating) {
-        head[i] = a.per_head.of(it), it -= head[i] * a.per_head.d;
-        turn[i] = it < a.turned;
-        ch[i] = turn[i] ? (N == 1 && !a.neox ? 2 * it : it * N) : 2 * a.half + (it - a.turned) * N;
-      } else {
-        it -= rotating;
-        const uint32_t h = a.per_v.of(it);
-        head[i] = a.heads + a.kv_heads + h, ch[i] = (it - h * a.per_v.d) * N, turn[i] = false;
-      }
-      const T* src = static_cast<const T*>(a.qkv) + (size_t)row[i] * a.stride + (size_t)head[i] * a.hd + ch[i];
-      load_run<T, N>(src, x[i]);
-      if (turn[i] && (a.neox || N == 1)) load_run<T, N>(src + apart, y[i]);
-      pos[i] = a.position[row[i]], slot[i] = a.slot[row[i]];
+  const bool adjacent = N == 1 && !a.neox; // a pair's second channel is the next one, and a piece of its own
+  for (uint32_t id = blockIdx.x * APPEND_THREADS + threadIdx.x; id < all; id += threads) {
+    const uint32_t row = a.items.of(id);
+    const int32_t pos = a.position[row];
+    const int64_t slot = a.slot[row];
+    uint32_t it = id - row * a.items.d, head, last; // this item's heads: head .. last - 1
+    uint32_t ch;                                    // the piece's first channel; a second one lies `apart` behind
+    bool turn = false;
+    if (it < a.turned_blocks * a.per_head.d) {
+      const uint32_t block = a.per_head.of(it);
+      it -= block * a.per_head.d, turn = it < a.turned;
+      head = block * H, last = a.heads + a.kv_heads;
+      ch = turn ? (adjacent ? 2 * it : it * N) : 2 * a.half + (it - a.turned) * N;
+    } else {
+      it -= a.turned_blocks * a.per_head.d;
+      const uint32_t block = a.per_v.of(it);
+      head = a.heads + a.kv_heads + block * H, last = a.heads + 2 * a.kv_heads, ch = (it - block * a.per_v.d) * N;
     }
+    const bool second = turn && (a.neox || N == 1);
+    const uint32_t apart = a.neox ? a.half : 1u, n = min((uint32_t)H, last - head);
+    const T* src = static_cast<const T*>(a.qkv) + (size_t)row * a.stride + (size_t)head * a.hd + ch;
+    float x[H][N], y[H][N];
 #pragma unroll
-    for (int i = 0; i < IN_FLIGHT; i++) {
-      if (first + i * threads >= all) break;
-      const bool dead = pos[i] < 0 || (a.half && (uint32_t)pos[i] >= a.positions);
-      const bool second = turn[i] && (a.neox || N == 1);
-      if (turn[i] && !dead) {
-        const float* c = a.cos + (size_t)pos[i] * a.half;
-        const float* s = a.sin + (size_t)pos[i] * a.half;
-        if (second) {
-          float cs[N], sn[N];
-          load_run<float, N>(c + (N == 1 && !a.neox ? ch[i] / 2 : ch[i]), cs), load_run<float, N>(s + (N == 1 && !a.neox ? ch[i] / 2 : ch[i]), sn);
+    for (int h = 0; h < H; h++)
+      if (h < n) {
+        load_run<T, N>(src + (size_t)h * a.hd, x[h]);
+        if (second) load_run<T, N>(src + (size_t)h * a.hd + apart, y[h]);
+      }
+    const bool dead = pos < 0 || (a.half && (uint32_t)pos >= a.positions);
+    if (turn && !dead) {
+      const size_t at = (size_t)pos * a.half;
+      if (second) {
+        float cs[N], sn[N];
+        load_run<float, N>(a.cos + at + (adjacent ? ch / 2 : ch), cs), load_run<float, N>(a.sin + at + (adjacent ? ch / 2 : ch), sn);
+#pragma unroll
+        for (int h = 0; h < H; h++)
 #pragma unroll
           for (int e = 0; e < N; e++) {
-            const float u = x[i][e], w = y[i][e];
-            x[i][e] = fmaf(u, cs[e], -(w * sn[e])), y[i][e] = fmaf(u, sn[e], w * cs[e]);
+            const float u = x[h][e], w = y[h][e];
+            x[h][e] = fmaf(u, cs[e], -(w * sn[e])), y[h][e] = fmaf(u, sn[e], w * cs[e]);
           }
-        } else if constexpr (N > 1) {
-          float cs[N / 2], sn[N / 2];
-          load_run<float, N / 2>(c + ch[i] / 2, cs), load_run<float, N / 2>(s + ch[i] / 2, sn);
+      } else if constexpr (N > 1) {
+        float cs[N / 2], sn[N / 2];
+        load_run<float, N / 2>(a.cos + at + ch / 2, cs), load_run<float, N / 2>(a.sin + at + ch / 2, sn);
+#pragma unroll
+        for (int h = 0; h < H; h++)
 #pragma unroll
           for (int e = 0; e < N / 2; e++) {
-            const float u = x[i][2 * e], w = x[i][2 * e + 1];
-            x[i][2 * e] = fmaf(u, cs[e], -(w * sn[e])), x[i][2 * e + 1] = fmaf(u, sn[e], w * cs[e]);
+            const float u = x[h][2 * e], w = x[h][2 * e + 1];
+            x[h][2 * e] = fmaf(u, cs[e], -(w * sn[e])), x[h][2 * e + 1] = fmaf(u, sn[e], w * cs[e]);
           }
-        }
       }
-      if (head[i] < a.heads) {
+    }
+    const bool stored = !dead && (uint64_t)slot < a.slots;
+    const uint64_t cache_at = (((uint64_t)slot >> a.page_shift) * a.kv_heads << a.page_shift) + ((uint64_t)slot & ((1u << a.page_shift) - 1));
+#pragma unroll
+    for (int h = 0; h < H; h++) {
+      if (h >= n) break;
+      const uint32_t now = head + h;
+      if (now < a.heads) {
         if (dead) {
 #pragma unroll
-          for (int e = 0; e < N; e++) x[i][e] = y[i][e] = 0.0f;
+          for (int e = 0; e < N; e++) x[h][e] = y[h][e] = 0.0f;
         }
-        T* to = static_cast<T*>(a.q_out) + (size_t)row[i] * a.q_stride + (size_t)head[i] * a.hd + ch[i];
-        store_run<T, N>(to, x[i]);
-        if (second) store_run<T, N>(to + apart, y[i]);
-      } else if (!dead && (uint64_t)slot[i] < a.slots) {
-        const bool is_k = head[i] < a.heads + a.kv_heads;
-        const uint32_t kh = head[i] - a.heads - (is_k ? 0 : a.kv_heads);
-        const uint64_t page = (uint64_t)slot[i] >> a.page_shift, in_page = (uint64_t)slot[i] & ((1u << a.page_shift) - 1);
-        C* to = static_cast<C*>(is_k ? a.k : a.v) + (((page * a.kv_heads + kh) << a.page_shift) + in_page) * a.hd + ch[i];
-        store_run<C, N>(to, x[i]);
-        if (second) store_run<C, N>(to + apart, y[i]);
+        T* to = static_cast<T*>(a.q_out) + (size_t)row * a.q_stride + (size_t)now * a.hd + ch;
+        store_run<T, N>(to, x[h]);
+        if (second) store_run<T, N>(to + apart, y[h]);
+      } else if (stored) {
+        const bool is_k = now < a.heads + a.kv_heads;
+        const uint32_t kh = now - a.heads - (is_k ? 0 : a.kv_heads);
+        C* to = static_cast<C*>(is_k ? a.k : a.v) + (cache_at + ((uint64_t)kh << a.page_shift)) * a.hd + ch;
+        store_run<C, N>(to, x[h]);
+        if (second) store_run<C, N>(to + apart, y[h]);
       }
     }
   }
+}
+
+// Many rows: a loading warp streams whole rows into shared memory with one bulk copy each, and the rows of the tables behind
+// them (position and slot are looked up 32 rows ahead, so that nothing waits for an address); each of the other warps owns a
+// stage, rotates its rows from shared memory and stores them. No load latency is left in the warps that store.
+constexpr int ROW_WARPS = 8 /* one per stage */, ROW_THREADS = ROW_WARPS * 32 + 32;
+constexpr uint32_t ROW_LEAST = 1024; // rows from which on this is the faster way
+constexpr uint32_t ROW_STAGES = 8, ROW_SHARED = 110 << 10, ROW_CTAS = 2;
+struct RowStage {
+  uint64_t full, empty;
+  int64_t slot;
+  int32_t pos;
+};
+
+template <typename T, typename C, int N>
+__global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) append_rows_kernel(AppendArgs a, uint32_t stages, uint32_t stage_bytes, uint32_t row_bytes, uint32_t table_bytes) {
+  extern __shared__ __align__(128) char raw[];
+  RowStage* stage_of = reinterpret_cast<RowStage*>(raw);
+  char* data = raw + 512;
+  static_assert(ROW_STAGES * sizeof(RowStage) <= 512 && ROW_STAGES <= ROW_WARPS, "the stages' heads lie in front, and each has its warp");
+  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (uint32_t s = 0; s < stages; s++) tc::mbar_init(&stage_of[s].full, 1), tc::mbar_init(&stage_of[s].empty, 1);
+    tc::fence_barrier_init();
+  }
+  __syncthreads();
+  grid_wait();
+  const uint32_t begin = (uint32_t)((uint64_t)a.rows * blockIdx.x / gridDim.x), end = (uint32_t)((uint64_t)a.rows * (blockIdx.x + 1) / gridDim.x);
+  uint32_t stage = 0, phase = 0;
+  bool alive = true;
+  if (warp == ROW_WARPS) {
+    int32_t pos = 0;
+    int64_t slot = 0;
+    for (uint32_t r = begin; r < end; r++) {
+      const uint32_t i = (r - begin) & 31;
+      if (i == 0 && r + lane < end) pos = a.position[r + lane], slot = a.slot[r + lane];
+      const int32_t p = __shfl_sync(0xffffffffu, pos, i);
+      const int64_t sl = __shfl_sync(0xffffffffu, slot, i);
+      if (lane == 0) {
+        RowStage& st = stage_of[stage];
+        if (alive && r - begin >= stages && !tc::mbar_wait(&st.empty, phase ^ 1)) {
+          alive = false;
+          atomicExch(a.err_flag, 1);
+        }
+        st.pos = p, st.slot = sl;
+        const bool turned = table_bytes && p >= 0 && (uint32_t)p < a.positions;
+        char* to = data + stage * stage_bytes;
+        tc::mbar_arrive_expect_tx(&st.full, row_bytes + (turned ? 2 * table_bytes : 0));
+        auto copy = [&](char* dst, const void* src, uint32_t bytes) {
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(tc::smem_u32(dst)), "l"(src),
+                       "r"(bytes), "r"(tc::smem_u32(&st.full))
+                       : "memory");
+        };
+        copy(to, static_cast<const T*>(a.qkv) + (size_t)r * a.stride, row_bytes);
+        if (turned) {
+          copy(to + row_bytes, a.cos + (size_t)p * a.half, table_bytes);
+          copy(to + row_bytes + table_bytes, a.sin + (size_t)p * a.half, table_bytes);
+        }
+      }
+      if (++stage == stages) stage = 0, phase ^= 1;
+    }
+    // (no copy is in flight when the CTA ends, whatever became of the others' waits)
+    for (uint32_t i = 0; lane == 0 && i < min(end - begin, stages); i++) {
+      if (stage == 0) stage = stages, phase ^= 1;
+      stage--;
+      if (!tc::mbar_wait(&stage_of[stage].full, phase)) atomicExch(a.err_flag, 2);
+    }
+    return;
+  }
+  for (uint32_t r = begin; r < end; r++) {
+    const uint32_t now = stage, ph = phase;
+    if (++stage == stages) stage = 0, phase ^= 1;
+    if (now != warp) continue; // (a warp per stage, so that it meets every phase of its barriers in order; fewer stages leave warps idle)
+    RowStage& st = stage_of[now];
+    if (alive && !tc::mbar_wait(&st.full, ph)) {
+      alive = false; // (reported; the results are wrong, the barriers stay whole)
+      if (lane == 0) atomicExch(a.err_flag, 3);
+    }
+    const T* row = reinterpret_cast<const T*>(data + now * stage_bytes);
+    const int32_t pos = st.pos;
+    const int64_t slot = st.slot;
+    const bool dead = pos < 0 || (a.half && (uint32_t)pos >= a.positions), stored = !dead && (uint64_t)slot < a.slots;
+    // (table rows that are no whole 16 bytes stay where they are)
+    const float* cos = table_bytes ? reinterpret_cast<const float*>(data + now * stage_bytes + row_bytes) : a.cos + (dead ? 0 : (size_t)pos * a.half);
+    const float* sin = table_bytes ? cos + a.half : a.sin + (dead ? 0 : (size_t)pos * a.half);
+    const bool adjacent = N == 1 && !a.neox;
+    const uint32_t apart = a.neox ? a.half : 1u;
+    const uint64_t cache_at = (((uint64_t)slot >> a.page_shift) * a.kv_heads << a.page_shift) + ((uint64_t)slot & ((1u << a.page_shift) - 1));
+    const uint32_t rotating = (a.heads + a.kv_heads) * a.per_head.d;
+#pragma unroll(N == 8 ? 2 : 4)
+    for (uint32_t id = lane; id < a.items.d; id += 32) {
+      uint32_t it = id, head, ch;
+      bool turn = false;
+      if (it < rotating) {
+        head = a.per_head.of(it), it -= head * a.per_head.d, turn = it < a.turned;
+        ch = turn ? (adjacent ? 2 * it : it * N) : 2 * a.half + (it - a.turned) * N;
+      } else {
+        it -= rotating;
+        const uint32_t h = a.per_v.of(it);
+        head = a.heads + a.kv_heads + h, ch = (it - h * a.per_v.d) * N;
+      }
+      const bool second = turn && (a.neox || N == 1);
+      float x[N], y[N];
+      load_run<T, N>(row + head * a.hd + ch, x);
+      if (second) {
+        load_run<T, N>(row + head * a.hd + ch + apart, y);
+        float cs[N], sn[N];
+        load_run<float, N>(cos + (adjacent ? ch / 2 : ch), cs), load_run<float, N>(sin + (adjacent ? ch / 2 : ch), sn);
+#pragma unroll
+        for (int e = 0; e < N; e++) {
+          const float u = x[e], w = y[e];
+          x[e] = fmaf(u, cs[e], -(w * sn[e])), y[e] = fmaf(u, sn[e], w * cs[e]);
+        }
+      } else if constexpr (N > 1) {
+        if (turn) {
+        float cs[N / 2], sn[N / 2];
+        load_run<float, N / 2>(cos + ch / 2, cs), load_run<float, N / 2>(sin + ch / 2, sn);
+#pragma unroll
+        for (int e = 0; e < N / 2; e++) {
+          const float u = x[2 * e], w = x[2 * e + 1];
+          x[2 * e] = fmaf(u, cs[e], -(w * sn[e])), x[2 * e + 1] = fmaf(u, sn[e], w * cs[e]);
+        }
+        }
+      }
+      if (head < a.heads) {
+        if (dead) {
+#pragma unroll
+          for (int e = 0; e < N; e++) x[e] = y[e] = 0.0f;
+        }
+        T* to = static_cast<T*>(a.q_out) + (size_t)r * a.q_stride + (size_t)head * a.hd + ch;
+        store_run<T, N>(to, x);
+        if (second) store_run<T, N>(to + apart, y);
+      } else if (stored) {
+        const bool is_k = head < a.heads + a.kv_heads;
+        const uint32_t kh = head - a.heads - (is_k ? 0 : a.kv_heads);
+        C* to = static_cast<C*>(is_k ? a.k : a.v) + (cache_at + ((uint64_t)kh << a.page_shift)) * a.hd + ch;
+        store_run<C, N>(to, x);
+        if (second) store_run<C, N>(to + apart, y);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) tc::mbar_arrive(&st.empty);
+  }
+}
+
+template <typename T, typename C, int N>
+int launch_rows(FcDevice* dev, const AppendArgs& a, uint32_t stages, uint32_t stage_bytes, uint32_t row_bytes, uint32_t table_bytes) {
+  auto kern = append_rows_kernel<T, C, N>;
+  static OncePerDevice once;
+  if (once.first(dev->ordinal)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ROW_SHARED);
+    if (e != cudaSuccess) once.again(dev->ordinal);
+    FC_CUDA(dev, e);
+  }
+  const uint32_t ctas = std::min(a.rows, (uint32_t)dev->prop.multiProcessorCount * ROW_CTAS);
+  FC_LAUNCH(dev, "paged_append", launch_on(dev, true, kern, dim3(ctas), dim3(ROW_THREADS), 512 + stages * stage_bytes, a, stages, stage_bytes, row_bytes,
+                                           table_bytes));
+  return FC_OK;
 }
 
 template <typename T, typename C>
@@ -180,11 +346,28 @@ int launch_append(FcDevice* dev, AppendArgs a, uint32_t rope_dim, bool aligned8,
   const uint32_t n = fits(8, aligned8) ? 8 : fits(4, aligned4) ? 4 : fits(2, aligned2) ? 2 : 1;
   a.turned = n == 1 ? a.half : (a.neox ? a.half : rope_dim) / n;
   a.per_head = div_by(a.turned + (a.hd - rope_dim) / n), a.per_v = div_by(a.hd / n);
-  const uint64_t items = (uint64_t)(a.heads + a.kv_heads) * a.per_head.d + (uint64_t)a.kv_heads * a.per_v.d;
+  const uint32_t table_bytes = a.half % 4 == 0 && aligned_to(a.cos, 16) && aligned_to(a.sin, 16) ? a.half * 4 : 0;
+  const uint32_t row_bytes = (a.heads + 2 * a.kv_heads) * a.hd * (uint32_t)sizeof(T), stage_bytes = (row_bytes + 2 * table_bytes + 127) / 128 * 128;
+  const uint32_t stages = std::min(ROW_STAGES, (ROW_SHARED - 512) / stage_bytes);
+  if (aligned_to(a.qkv, 16) && a.stride * sizeof(T) % 16 == 0 && stages >= 3 && a.rows >= ROW_LEAST && n != 2) {
+    a.items = div_by((a.heads + a.kv_heads) * a.per_head.d + a.kv_heads * a.per_v.d);
+    return n == 8   ? launch_rows<T, C, 8>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
+           : n == 4 ? launch_rows<T, C, 4>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
+           : n == 2 ? launch_rows<T, C, 2>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
+                    : launch_rows<T, C, 1>(dev, a, stages, stage_bytes, row_bytes, table_bytes);
+  }
+  // four heads a thread, unless the pieces of single heads do not even fill the SMs
+  auto count = [&](uint32_t h) { return (uint64_t)((a.heads + a.kv_heads + h - 1) / h) * a.per_head.d + (uint64_t)((a.kv_heads + h - 1) / h) * a.per_v.d; };
+  const bool many = n > 1 && a.rows * count(1) >= (uint64_t)dev->prop.multiProcessorCount * 2048;
+  const uint64_t items = count(many ? 4 : 1);
+  a.turned_blocks = many ? (a.heads + a.kv_heads + 3) / 4 : a.heads + a.kv_heads;
   // (items are counted in 31 bits: more rows go in several launches)
   const uint32_t at_once = (uint32_t)std::min<uint64_t>(a.rows, 0x7fffffffull / items);
   a.items = div_by((uint32_t)items);
-  auto kern = n == 8 ? append_kernel<T, C, 8> : n == 4 ? append_kernel<T, C, 4> : n == 2 ? append_kernel<T, C, 2> : append_kernel<T, C, 1>;
+  auto kern = n == 8   ? (many ? append_kernel<T, C, 8, 4> : append_kernel<T, C, 8, 1>)
+              : n == 4 ? (many ? append_kernel<T, C, 4, 4> : append_kernel<T, C, 4, 1>)
+              : n == 2 ? (many ? append_kernel<T, C, 2, 4> : append_kernel<T, C, 2, 1>)
+                       : append_kernel<T, C, 1, 1>;
   const uint32_t rows = a.rows;
   for (uint32_t r = 0; r < rows; r += at_once) {
     AppendArgs b = a;
@@ -237,6 +420,7 @@ FC_API int fc_paged_append_dev(FcDevice* dev, const FcPagedCache* c, const FcRot
   if (!rows) return FC_OK;
   if (rows > (1u << 30)) return fc_fail(dev, FC_ERR_SHAPE, "%u rows", rows);
   a.qkv = qkv, a.q_out = q_out, a.k = c->k, a.v = c->v, a.slot = slot, a.position = position, a.stride = stride, a.q_stride = q_stride;
+  a.err_flag = dev->d_flag;
   a.rows = rows, a.slots = (uint64_t)c->n_pages * c->page, a.heads = heads, a.kv_heads = c->kv_heads, a.hd = c->head_dim;
   a.page_shift = (uint32_t)__builtin_ctz(c->page);
   const uint32_t rope_dim = 2 * a.half;

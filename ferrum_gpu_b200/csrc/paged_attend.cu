@@ -363,14 +363,18 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     for (uint32_t tile = w.tile; tile < tile_end; tile++) {
       const uint32_t now = stage, ph = phase;
       if (++stage == STAGES) stage = 0, phase ^= 1;
+      // Other groups' tiles are waited for too: a parity tells two neighbouring phases of a stage apart, so a warp must not come
+      // to a stage's next phase before it has seen this one end. (No stage gets two phases ahead of a warp that waits here:
+      // GROUPS <= STAGES, and the stage of its own next tile is not refilled.)
+      static_assert(S::GROUPS <= STAGES, "a warp meets every phase of every stage");
+      if (alive && !tc::mbar_wait(&full[now], ph)) {
+        alive = false; // (reported; the results are wrong, the barriers stay whole)
+        if (lane == 0) atomicExch(a.err_flag, 3);
+      }
       if (S::GROUPS > 1) {
         const bool ours = turn == group;
         turn = turn + 1 == S::GROUPS ? 0 : turn + 1;
         if (!ours) continue;
-      }
-      if (alive && !tc::mbar_wait(&full[now], ph)) {
-        alive = false; // (reported; the results are wrong, the barriers stay whole)
-        if (lane == 0) atomicExch(a.err_flag, 3);
       }
       const uint32_t p = tile * TP + sub * PS;
       if (p < w.len) {

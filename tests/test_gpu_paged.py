@@ -246,6 +246,14 @@ def test_append_strides_and_alignments(dev, kw, act, neox):
     _append_case(dev, 33, 6, 2, 64, 32, neox, act, "bf16" if act == "bf16" else "f32", 16, seed=6, **kw)
 
 
+@pytest.mark.parametrize("act,cache", [("f32", "f32"), ("f32", "f16"), ("bf16", "bf16"), ("f16", "f32")])
+@pytest.mark.parametrize("heads,kv,hd,rope_dim", [(12, 4, 64, 64), (32, 8, 128, 96), (3, 1, 40, 24), (64, 8, 128, 128), (6, 6, 64, 0), (56, 8, 256, 256), (2, 2, 64, 40)])
+@pytest.mark.parametrize("neox", [False, True])
+def test_append_many_rows(dev, act, cache, heads, kv, hd, rope_dim, neox):
+    """Rows from narrow (a few hundred bytes) to wide (tens of KB), more than there are CTAs; with rows that are no tokens."""
+    _append_case(dev, 2500 if heads * hd < 8192 else 1100, heads, kv, hd, rope_dim, neox, act, cache, 16, seed=7, pad=8 if heads == 12 else 0, q_pad=16 if heads == 6 else 0)
+
+
 # ---- attention ----------------------------------------------------------------------------------------------------------
 
 def _attend_case(dev, lens, heads, kv, hd, act, cache, page, scale=0.0, request=None, q_scale=2.0, seed=0, pad=0, shift=0, holes=(), n_pages=None, poison=True):
