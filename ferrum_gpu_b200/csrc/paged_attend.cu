@@ -34,7 +34,7 @@
 namespace {
 
 constexpr int WARPS = 4, ROWS8 = 8; // multiplying warps of a CTA (one more loads), heads of one matrix operand
-constexpr int THREADS = WARPS * 32 + 32;
+constexpr int THREADS = WARPS * 32 + 64; // and one that loads, one that writes results
 constexpr float P_LIFT = 10.0f;
 
 struct AttendArgs {
@@ -115,10 +115,25 @@ __device__ __forceinline__ uint32_t spread(uint32_t c) { return (c & 1) << 2 | c
 __device__ __forceinline__ float load_act(const void* p, int act, size_t i) {
   return act == FC_F32 ? static_cast<const float*>(p)[i] : act == FC_F16 ? to_f32(static_cast<const __half*>(p)[i]) : to_f32(static_cast<const __nv_bfloat16*>(p)[i]);
 }
-__device__ __forceinline__ void store_act(void* p, int act, size_t i, float v) {
-  if (act == FC_F32) static_cast<float*>(p)[i] = v;
-  else if (act == FC_F16) static_cast<__half*>(p)[i] = __float2half_rn(v);
-  else static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
+// four elements side by side; `wide`: their address is a multiple of what they take
+__device__ __forceinline__ void store_four(void* p, int act, bool wide, size_t i, const float4& v) {
+  if (act == FC_F32) {
+    float* to = static_cast<float*>(p) + i;
+    if (wide) *reinterpret_cast<float4*>(to) = v;
+    else to[0] = v.x, to[1] = v.y, to[2] = v.z, to[3] = v.w;
+    return;
+  }
+  union {
+    uint2 all;
+    __half h[4];
+    __nv_bfloat16 b[4];
+    unsigned short u[4];
+  } x;
+  if (act == FC_F16) x.h[0] = __float2half_rn(v.x), x.h[1] = __float2half_rn(v.y), x.h[2] = __float2half_rn(v.z), x.h[3] = __float2half_rn(v.w);
+  else x.b[0] = __float2bfloat16_rn(v.x), x.b[1] = __float2bfloat16_rn(v.y), x.b[2] = __float2bfloat16_rn(v.z), x.b[3] = __float2bfloat16_rn(v.w);
+  unsigned short* to = static_cast<unsigned short*>(p) + i;
+  if (wide) *reinterpret_cast<uint2*>(to) = x.all;
+  else to[0] = x.u[0], to[1] = x.u[1], to[2] = x.u[2], to[3] = x.u[3];
 }
 
 // positions a row sees, and the row of the table they are found in
@@ -139,10 +154,12 @@ struct Shape {
   static constexpr int PS = F32 && HDP > 64 ? 8 : 16;                    // positions of a warp's step
   static constexpr int SHARE = TP / PS, GROUPS = WARPS / SHARE;          // warps that share a tile; groups that take tiles in turn
   static constexpr uint32_t HALF = TP * BOXES * 128, STAGE = 2 * HALF;   // bytes of k (or v), of both
-  static constexpr int CTAS = HDP == 64 && !F32 ? 3 : 2;                 // resident on an SM
-  static constexpr int STAGES = HDP == 256 ? 5 : HDP == 64 && !F32 ? 4 : 3;
-  static constexpr uint32_t Q_BYTES = HDP / (4 * E) * 3 * 32 * 16, JOIN_BYTES = 2 * ROWS8 * HDP * 4;
-  static constexpr uint32_t SHARED = STAGES * STAGE + (Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES);
+  static constexpr int CTAS = 2;                                         // resident on an SM
+  static constexpr int STAGES = HDP == 256 ? 5 : HDP == 64 && !F32 ? 6 : 3;
+  static constexpr int Q_TERMS = F32 ? 2 : 3;
+  static constexpr uint32_t Q_BYTES = HDP / (4 * E) * Q_TERMS * 32 * 16, JOIN_BYTES = 2 * ROWS8 * HDP * 4, DONE_BYTES = ROWS8 * HDP * 4;
+  static constexpr uint32_t Q_OR_JOIN = Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES;
+  static constexpr uint32_t SHARED = STAGES * STAGE + Q_OR_JOIN + DONE_BYTES;
   static constexpr uint32_t BYTES = SHARED + 1024; // (tiles begin on whole swizzle patterns)
 };
 
@@ -177,17 +194,21 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
   extern __shared__ char raw[];
   __shared__ float sm_m[WARPS][ROWS8], sm_l[WARPS][ROWS8];
   __shared__ uint32_t sm_big[ROWS8];
-  __shared__ uint32_t sm_scan[WARPS + 1], sm_row, sm_at, sm_last;
-  __shared__ uint64_t full[STAGES], empty[STAGES];
+  __shared__ uint32_t sm_scan[WARPS + 2], sm_row, sm_at, sm_n_late;
+  __shared__ uint64_t full[STAGES], empty[STAGES], done_full, done_empty, all_done;
+  __shared__ float done_m[ROWS8], done_l[ROWS8];
+  __shared__ struct { uint32_t first_tile, tiles, r, h0, heads; } sm_late[2]; // segments to be joined by this CTA
   __shared__ unsigned long long held[STAGES]; // of a tile: which of its pages are pages
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t stages = (tc::smem_u32(raw) + 1023) & ~1023u;
   char* shared = raw + (stages - tc::smem_u32(raw)) + STAGES * S::STAGE;
-  uint4 (*sm_q)[3][32] = reinterpret_cast<uint4 (*)[3][32]>(shared);      // q's terms while positions are multiplied,
-  float (*sm_o)[ROWS8][HDP] = reinterpret_cast<float (*)[ROWS8][HDP]>(shared); // then what two warps hand to the others
+  uint4 (*sm_q)[S::Q_TERMS][32] = reinterpret_cast<uint4 (*)[S::Q_TERMS][32]>(shared); // q's terms while positions are multiplied,
+  float (*sm_o)[ROWS8][HDP] = reinterpret_cast<float (*)[ROWS8][HDP]>(shared);         // then what two warps hand to the others
+  float (*sm_done)[HDP] = reinterpret_cast<float (*)[HDP]>(shared + S::Q_OR_JOIN);     // a segment's result, for the warp that writes it
   const uint32_t per_row = a.kv_heads * a.blocks;
   if (tid == 0) {
     for (int s = 0; s < STAGES; s++) tc::mbar_init(&full[s], 1), tc::mbar_init(&empty[s], S::SHARE);
+    for (uint64_t* bar : {&done_full, &done_empty, &all_done}) tc::mbar_init(bar, 1);
     tc::fence_barrier_init();
   }
   grid_wait();
@@ -206,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
   __syncthreads();
   uint32_t all = 0;
 #pragma unroll
-  for (int w = 0; w <= WARPS; w++) {
+  for (int w = 0; w < WARPS + 2; w++) {
     if (w < (int)warp) upto += sm_scan[w];
     all += sm_scan[w];
   }
@@ -214,6 +235,13 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
   const uint32_t n_cta = min(gridDim.x, all), share = all / n_cta, extra = all % n_cta; // (the first `extra` CTAs take one more)
   if (blockIdx.x >= n_cta) return;
   auto begin_of = [&](uint32_t c) { return c * share + min(c, extra); };
+  auto owner_of = [&](uint32_t tile) {
+    const uint32_t longer = extra * (share + 1);
+    return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+  };
+  auto part_of = [&](uint32_t c, uint32_t first_tile) { // a CTA has two: one for where it begins, one for where it ends
+    return a.parts + (size_t)(2 * c + (begin_of(c) >= first_tile ? 0 : 1)) * part_floats(HDP);
+  };
   const uint32_t begin = begin_of(blockIdx.x), end = begin_of(blockIdx.x + 1);
   if (upto - mine <= begin && begin < upto) {
     uint32_t at = upto - mine, r = r0;
@@ -290,37 +318,97 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     return;
   }
 
+  if (warp == WARPS + 1) {
+    // ---- the writing warp: a segment's result to the caller, or as a part of it to the one that joins the parts; the others
+    // are already at the next segment. Lane i has four channels of a head, 128 further on, .. ----
+    constexpr int OWN = ROWS8 * HDP / 128;
+    const bool wide = (((uintptr_t)a.out | a.out_stride * (a.act == FC_F32 ? 4 : 2)) & 15) == 0;
+    uint32_t n = 0, late = 0;
+    for (; w.at < end; n++) {
+      const uint32_t tile_end = min(w.tiles, w.tile + (end - w.at));
+      const uint32_t kvh = w.which / a.blocks, h0 = kvh * a.group + (w.which % a.blocks) * ROWS8;
+      const uint32_t heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
+      const bool whole = w.tile == 0 && tile_end == w.tiles;
+      const uint32_t first_tile = w.row_at + w.which * w.tiles;
+      if (!tc::mbar_wait(&done_full, n & 1) && lane == 0) atomicExch(a.err_flag, 4);
+      float4 v[OWN];
+#pragma unroll
+      for (int i = 0; i < OWN; i++) v[i] = *(reinterpret_cast<const float4*>(&sm_done[0][0]) + lane + 32 * i);
+      const float m = done_m[lane % ROWS8], l = done_l[lane % ROWS8];
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&done_empty);
+      if (whole) {
+        const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+        for (int i = 0; i < OWN; i++) {
+          const uint32_t at = lane + 32 * i, h = at / (HDP / 4), ch = at % (HDP / 4) * 4;
+          const float fh = __shfl_sync(0xffffffffu, f, h);
+          if (h < heads && ch < a.hd)
+            store_four(a.out, a.act, wide, (size_t)w.r * a.out_stride + (size_t)(h0 + h) * a.hd + ch, make_float4(v[i].x * fh, v[i].y * fh, v[i].z * fh, v[i].w * fh));
+        }
+      } else {
+        float* part = part_of(blockIdx.x, first_tile);
+        if (lane < ROWS8) part[lane] = m, part[ROWS8 + lane] = l;
+#pragma unroll
+        for (int i = 0; i < OWN; i++) *(reinterpret_cast<float4*>(part + 2 * ROWS8) + lane + 32 * i) = v[i];
+        __syncwarp();
+        if (lane == 0) { // (the warp's barriers and the one that ends this loop carry the fences' order to the others)
+          const uint32_t c0 = owner_of(first_tile), c1 = owner_of(first_tile + w.tiles - 1);
+          __threadfence();
+          if (atomicAdd(&a.arrived[c0], 1u) == c1 - c0) {
+            a.arrived[c0] = 0; // for the next call
+            sm_late[late++] = {first_tile, w.tiles, w.r, h0, heads};
+          }
+          __threadfence();
+        }
+      }
+      next_segment<TP>(a, per_row, tile_end, w);
+    }
+    if (lane == 0) {
+      sm_n_late = late;
+      tc::mbar_arrive(&all_done);
+    }
+    return;
+  }
+
   // ---- the multiplying warps ----
   const uint32_t g = lane >> 2, t = lane & 3, sub = warp % S::SHARE, group = warp / S::SHARE;
   // where this lane's pieces lie in a tile: row i of eight is swizzled by i
   const uint32_t k_at = (sub * PS + spread(g)) * 128 + ((t ^ spread(g)) << 4);
   const uint32_t v_at = S::HALF + (sub * PS + t) * 128 + ((spread(g) ^ t) << 4);
-  uint32_t stage = 0, phase = 0, turn = 0;
+  uint32_t stage = 0, phase = 0, turn = 0, segment = 0;
   bool alive = true;
-  while (w.at < end) {
-    const uint32_t tile_end = min(w.tiles, w.tile + (end - w.at));
-    const uint32_t kvh = w.which / a.blocks, h0 = kvh * a.group + (w.which % a.blocks) * ROWS8;
-    const uint32_t heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
-    // q's terms as the matrix operand wants them: lane (g, t) of piece j has channels (4 j + t) E .. of head h0 + g
-    if (SIZED) { // (the f16 terms of a head: of q divided by a power of two near its largest)
-      if (tid < ROWS8) sm_big[tid] = 0;
-      warps_sync();
-    }
-    float mul = a.scale;
-    constexpr int ITEMS = (NJ * 32 + WARPS * 32 - 1) / (WARPS * 32);
-    float qv[ITEMS][E];
+  // q of a segment, fetched while the one before is multiplied: lane (g, t) of piece j has channels (4 j + t) E .. of head h0 + g
+  constexpr int ITEMS = (NJ * 32 + WARPS * 32 - 1) / (WARPS * 32);
+  float qv[ITEMS][E];
+  auto fetch_q = [&](const Walk& w) {
+    const uint32_t kvh = w.which / a.blocks, h0 = kvh * a.group + (w.which % a.blocks) * ROWS8, heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
 #pragma unroll
     for (int it = 0; it < ITEMS; it++) {
       const uint32_t id = tid + it * WARPS * 32, j = id / 32;
       if (NJ * 32 % (WARPS * 32) && id >= NJ * 32) continue;
-      float big = 0.0f;
 #pragma unroll
       for (int e = 0; e < E; e++) {
         const uint32_t ch = (4 * j + t) * E + e;
         qv[it][e] = g < heads && ch < a.hd ? load_act(a.q, a.act, (size_t)w.r * a.q_stride + (size_t)(h0 + g) * a.hd + ch) : 0.0f;
-        big = fmaxf(big, fabsf(qv[it][e]));
       }
-      if (SIZED) atomicMax(&sm_big[g], __float_as_uint(big));
+    }
+  };
+  fetch_q(w);
+  while (w.at < end) {
+    const uint32_t tile_end = min(w.tiles, w.tile + (end - w.at));
+    // q's terms as the matrix operand wants them (the f16 terms of a head: of q divided by a power of two near its largest)
+    if (SIZED && tid < ROWS8) sm_big[tid] = 0;
+    warps_sync(); // (the segment before has left the shared memory)
+    float mul = a.scale;
+    if (SIZED) {
+#pragma unroll
+      for (int it = 0; it < ITEMS; it++) {
+        float big = 0.0f;
+#pragma unroll
+        for (int e = 0; e < E; e++) big = fmaxf(big, fabsf(qv[it][e]));
+        if (NJ * 32 % (WARPS * 32) == 0 || tid + it * WARPS * 32 < NJ * 32) atomicMax(&sm_big[g], __float_as_uint(big));
+      }
     }
     float down = 1.0f;
     if (SIZED) {
@@ -351,6 +439,10 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
       for (int m = 0; m < TERMS; m++) sm_q[j][m][lane] = make_uint4(q[m][0], q[m][1], q[m][2], q[m][3]);
     }
     warps_sync();
+
+    Walk ahead = w;
+    next_segment<TP>(a, per_row, tile_end, ahead);
+    if (ahead.at < end) fetch_q(ahead);
 
     float o[NI][E][4], top = -INFINITY, sum = 0.0f; // of head g: the maximum is the lane's four's, the sum its own positions'
 #pragma unroll
@@ -542,113 +634,95 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     __syncwarp();
     if (warp == 1) give(1);
     warps_sync();
-    const bool whole = w.tile == 0 && tile_end == w.tiles;
-    const uint32_t first_tile = w.row_at + w.which * w.tiles;
-    auto part_of = [&](uint32_t c) { // a CTA has two: one for where it begins, one for where it ends
-      return a.parts + (size_t)(2 * c + (begin_of(c) >= first_tile ? 0 : 1)) * part_floats(HDP);
-    };
     if (warp == 0) {
       take(1);
-      if (whole) {
-        const float f = sum == 0.0f ? 0.0f : 1.0f / sum;
-        if (g < heads) {
-          const size_t at = (size_t)w.r * a.out_stride + (size_t)(h0 + g) * a.hd;
+      if (segment && !tc::mbar_wait(&done_empty, (segment - 1) & 1) && lane == 0) atomicExch(a.err_flag, 5);
 #pragma unroll
-          for (int i = 0; i < NI; i++)
+      for (int i = 0; i < NI; i++)
 #pragma unroll
-            for (int x = 0; x < 2; x++)
+        for (int x = 0; x < 2; x++)
 #pragma unroll
-              for (int e = 0; e < E; e++)
-                if ((8 * i + 4 * x) * E + ch0 + e < a.hd) store_act(a.out, a.act, at + (8 * i + 4 * x) * E + ch0 + e, o[i][e][x] * f);
-        }
-      } else {
-        float* part = part_of(blockIdx.x);
-        if (t == 0) part[g] = top, part[ROWS8 + g] = sum;
-#pragma unroll
-        for (int i = 0; i < NI; i++)
-#pragma unroll
-          for (int x = 0; x < 2; x++)
-#pragma unroll
-            for (int e = 0; e < E; e += 4)
-              *reinterpret_cast<float4*>(part + 2 * ROWS8 + g * HDP + (8 * i + 4 * x) * E + ch0 + e) =
-                  make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
-      }
+          for (int e = 0; e < E; e += 4)
+            *reinterpret_cast<float4*>(&sm_done[g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
+      if (t == 0) done_m[g] = top, done_l[g] = sum;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(&done_full);
     }
-    if (!whole) {
-      auto owner_of = [&](uint32_t tile) {
-        const uint32_t longer = extra * (share + 1);
-        return tile < longer ? tile / (share + 1) : extra + (tile - longer) / share;
+    segment++;
+    w = ahead;
+  }
+
+  // ---- the segments whose last part this CTA has written, joined by all four warps ----
+  if (!tc::mbar_wait(&all_done, 0)) {
+    if (lane == 0) atomicExch(a.err_flag, 6);
+    return; // (each warp by itself: without the verdict none of them may go on, and none waits for another)
+  }
+  for (uint32_t n = 0; n < sm_n_late; n++) {
+    // Thread (part k of 16, head) weighs its parts; every thread adds up its channels, the first parts' values in flight
+    // before the weights are known.
+    constexpr int PARTS = WARPS * 32 / ROWS8, OWN = (ROWS8 * HDP / 4 + WARPS * 32 - 1) / (WARPS * 32), EARLY = OWN == 4 ? 4 : 8;
+    float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(shared);
+    const uint32_t first_tile = sm_late[n].first_tile, c0 = owner_of(first_tile), parts = owner_of(first_tile + sm_late[n].tiles - 1) - c0 + 1;
+    const uint32_t heads = sm_late[n].heads, k0 = tid / ROWS8, head = tid % ROWS8;
+    auto part = [&](uint32_t k) { return part_of(c0 + k, first_tile); };
+    float m0 = k0 < parts ? __ldcg(part(k0) + head) : -INFINITY, l0 = k0 < parts ? __ldcg(part(k0) + ROWS8 + head) : 0.0f;
+    float4 early[OWN][EARLY];
+#pragma unroll
+    for (int i = 0; i < OWN; i++)
+#pragma unroll
+      for (int k = 0; k < EARLY; k++)
+        if (k < parts && tid + i * WARPS * 32 < ROWS8 * HDP / 4) early[i][k] = __ldcg(reinterpret_cast<const float4*>(part(k) + 2 * ROWS8) + tid + i * WARPS * 32);
+    float top = m0;
+#pragma unroll 4
+    for (uint32_t k = k0 + PARTS; k < parts; k += PARTS) top = fmaxf(top, __ldcg(part(k) + head));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+    if (lane < ROWS8) sm_m[warp][lane] = top;
+    warps_sync();
+    top = fmaxf(fmaxf(sm_m[0][head], sm_m[1][head]), fmaxf(sm_m[2][head], sm_m[3][head]));
+    if (top == -INFINITY) top = 0.0f;
+    float4 v[OWN];
+    float l[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; i++) v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l[i] = 0.0f;
+    for (uint32_t k1 = 0; k1 < parts; k1 += PARTS) {
+      const uint32_t k = k1 + k0, here = min((uint32_t)PARTS, parts - k1);
+      if (k1) m0 = k < parts ? __ldcg(part(k) + head) : -INFINITY, l0 = k < parts ? __ldcg(part(k) + ROWS8 + head) : 0.0f;
+      const float f = ex2(m0 - top);
+      sm_w[k0][head] = f, sm_w[PARTS + k0][head] = f * l0;
+      warps_sync();
+      auto add = [&](int i, uint32_t h, uint32_t k, const float4& x) {
+        const float f = sm_w[k][h];
+        v[i].x = fmaf(x.x, f, v[i].x), v[i].y = fmaf(x.y, f, v[i].y), v[i].z = fmaf(x.z, f, v[i].z), v[i].w = fmaf(x.w, f, v[i].w);
+        l[i] += sm_w[PARTS + k][h];
       };
-      const uint32_t c0 = owner_of(first_tile), c1 = owner_of(first_tile + w.tiles - 1);
-      if (warp == 0) { // (the part is this warp's own; the barriers carry the fences' order to the others)
-        __syncwarp();
-        if (lane == 0) {
-          __threadfence();
-          sm_last = atomicAdd(&a.arrived[c0], 1u) == c1 - c0;
-          __threadfence();
+#pragma unroll
+      for (int i = 0; i < OWN; i++) {
+        const uint32_t at = tid + i * WARPS * 32, h = at / (HDP / 4);
+        if (h >= heads) continue;
+        if (k1 == 0) {
+#pragma unroll
+          for (int k = 0; k < EARLY; k++)
+            if (k < here) add(i, h, k, early[i][k]);
         }
+#pragma unroll 8
+        for (uint32_t k = k1 ? 0 : EARLY; k < here; k++) add(i, h, k, __ldcg(reinterpret_cast<const float4*>(part(k1 + k) + 2 * ROWS8) + at));
       }
       warps_sync();
-      if (sm_last) {
-        // Each warp finds two heads' maxima over the parts; then, JOIN parts at a time, their weights go to shared memory and
-        // every thread adds its channels' values, all loads of a turn in flight together.
-        float (*sm_w)[ROWS8] = reinterpret_cast<float (*)[ROWS8]>(shared);
-        constexpr int JOIN = 32, OWN = (ROWS8 * HDP / 4 + WARPS * 32 - 1) / (WARPS * 32);
-        {
-          const uint32_t h = warp * 2 + (lane >> 4);
-          float m = -INFINITY;
-          for (uint32_t c = c0 + (lane & 15); c <= c1; c += 16) m = fmaxf(m, __ldcg(part_of(c) + h));
-#pragma unroll
-          for (int o = 8; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          sm_m[0][h] = m == -INFINITY ? 0.0f : m; // (all lanes of a head write the same)
-        }
-        warps_sync();
-        float4 v[OWN];
-        float l[OWN];
-#pragma unroll
-        for (int n = 0; n < OWN; n++) v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f), l[n] = 0.0f;
-        for (uint32_t c = c0; c <= c1; c += JOIN) {
-          const uint32_t here = min((uint32_t)JOIN, c1 - c + 1);
-          for (uint32_t i = tid; i < here * ROWS8; i += WARPS * 32) {
-            const uint32_t h = i % ROWS8;
-            const float* q = part_of(c + i / ROWS8);
-            const float f = ex2(__ldcg(q + h) - sm_m[0][h]);
-            sm_w[i / ROWS8][h] = f, sm_w[JOIN + i / ROWS8][h] = f * __ldcg(q + ROWS8 + h);
-          }
-          warps_sync();
-#pragma unroll
-          for (int n = 0; n < OWN; n++) {
-            const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
-            if (h >= heads || ch >= a.hd) continue;
-            const float* q = a.parts + 2 * ROWS8 + h * HDP + ch;
-#pragma unroll 8
-            for (uint32_t k = 0; k < here; k++) {
-              const float4 x = __ldcg(reinterpret_cast<const float4*>(q + (part_of(c + k) - a.parts)));
-              const float f = sm_w[k][h];
-              v[n].x = fmaf(x.x, f, v[n].x), v[n].y = fmaf(x.y, f, v[n].y), v[n].z = fmaf(x.z, f, v[n].z), v[n].w = fmaf(x.w, f, v[n].w);
-              l[n] += sm_w[JOIN + k][h];
-            }
-          }
-          warps_sync();
-        }
-#pragma unroll
-        for (int n = 0; n < OWN; n++) {
-          const uint32_t i = tid + n * WARPS * 32, h = i / (HDP / 4), ch = i % (HDP / 4) * 4;
-          if (h >= heads || ch >= a.hd) continue;
-          const float f = l[n] == 0.0f ? 0.0f : 1.0f / l[n];
-          const float x[4] = {v[n].x * f, v[n].y * f, v[n].z * f, v[n].w * f};
-#pragma unroll
-          for (int e = 0; e < 4; e++) store_act(a.out, a.act, (size_t)w.r * a.out_stride + (size_t)(h0 + h) * a.hd + ch + e, x[e]);
-        }
-        if (tid == 0) a.arrived[c0] = 0; // for the next call
-      }
     }
-    warps_sync(); // shared memory is free again
-    next_segment<TP>(a, per_row, tile_end, w);
+    const bool wide = (((uintptr_t)a.out | a.out_stride * (a.act == FC_F32 ? 4 : 2)) & 15) == 0;
+#pragma unroll
+    for (int i = 0; i < OWN; i++) {
+      const uint32_t at = tid + i * WARPS * 32, h = at / (HDP / 4), ch = at % (HDP / 4) * 4;
+      if (h >= heads || ch >= a.hd) continue;
+      const float f = l[i] == 0.0f ? 0.0f : 1.0f / l[i];
+      store_four(a.out, a.act, wide, (size_t)sm_late[n].r * a.out_stride + (size_t)(sm_late[n].h0 + h) * a.hd + ch,
+                 make_float4(v[i].x * f, v[i].y * f, v[i].z * f, v[i].w * f));
+    }
   }
 }
 
-constexpr uint32_t MAX_CTAS_PER_SM = 3;
+constexpr uint32_t MAX_CTAS_PER_SM = 2;
 
 template <typename C>
 bool cache_map(CUtensorMap* map, const void* p, const FcPagedCache* c, uint32_t tile) {
