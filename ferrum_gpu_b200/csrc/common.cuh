@@ -44,7 +44,7 @@ struct FcDevice {
   Workspace scratch;
   uint32_t weights = 0; // stand-alone weights alive
   cudaMemPool_t workspaces = nullptr;
-  ServingScratch attend, logprobs; // of the operators of a paged cache, from their first call on
+  ServingScratch attend, logprobs, plan; // of the operators of a paged cache, from their first call on
   int* d_flag = nullptr;   // device int for kernels that report a status
   int matvec_choice = 0;   // fc_debug_matvec_kernel: which kernel multiplies 1..8 rows (0: the library's rule)
   // per-kernel timing (off by default): one event pair per launch, summed by name on report

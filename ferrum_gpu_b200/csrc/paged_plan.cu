@@ -5,8 +5,12 @@
 // j-th of them being free[n_free - 1 - (need_0 + .. + need_{i-1} + j)]; row t of request i has position o_i + t - start_i.
 // Nothing depends on the order in which threads run.
 //
-// One cluster: each CTA forms the prefix sums of all requests for itself (a few KB from L2), then writes its share of the
-// rows. Only in-place updates (lengths, stack height) have to wait until every CTA has read, which is the cluster's barrier.
+// What bounds a step is latency: every CTA forms the prefix sums of all requests for itself (a few KB from L2) and writes its
+// share of the rows, four neighbouring rows a thread: one search for the request of the first, then onwards. A row that is the
+// first of a new page writes the table's entry. Pages that are given back go the same way, to the places above the stack's
+// height, which mean nothing until the height moves. Only what may be updated in place or has to wait for everybody's
+// consent (lengths, stack height) comes last: the CTA that arrives last writes it.
+#include <algorithm>
 #include <climits>
 #include <cmath>
 
@@ -15,20 +19,43 @@
 namespace {
 
 constexpr uint32_t PLAN_THREADS = 1024;
-constexpr uint32_t PLAN_MAX = 8192; // requests of a call: their prefix sums lie in shared memory (16 bytes each)
-constexpr uint32_t PLAN_CTAS = 8;   // CTAs of the cluster, where there are rows for them
+constexpr uint32_t PLAN_MAX = 8192;   // requests of a call: their prefix sums lie in shared memory (16 bytes each)
+constexpr uint32_t ROWS_AT_ONCE = 4;  // rows (or pages given back) of a thread
 
 struct PlanArgs {
   uint32_t page_shift, n_pages, requests, max_pages, n, rows;
+  bool vectors; // the rows' buffers lie on 16 bytes
   int32_t *table, *lens, *free, *n_free;
   const int32_t *req, *grow;
   int32_t* starts;
   int64_t* slot;
   int32_t *position, *request, *lens_out, *n_free_out, *status;
+  uint32_t* arrived; // and, behind it, whether a page given back is none
 };
 
-__device__ __forceinline__ void cluster_barrier() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+// Whether this CTA is the last of the grid to come here; what the others wrote before is visible to it then.
+__device__ __forceinline__ bool arrive_last(uint32_t* arrived) {
+  __shared__ int last;
+  __syncthreads();
+  if (gridDim.x == 1) return true;
+  if (threadIdx.x == 0) {
+    __threadfence();
+    last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+    if (last) *arrived = 0; // for the next call
+    __threadfence();
+  }
+  __syncthreads();
+  return last;
+}
+// The first of `n` entries whose running total lies above t.
+__device__ __forceinline__ uint32_t find(const int4* entry, uint32_t n, uint32_t t) {
+  uint32_t lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    if ((uint32_t)entry[mid].x > t) hi = mid;
+    else lo = mid + 1;
+  }
+  return lo;
 }
 
 // exclusive prefix sums of two 64-bit values per thread over the CTA, and their totals
@@ -64,7 +91,7 @@ __device__ __forceinline__ Pair scan_pair(Pair v, Pair& total) {
 __device__ __forceinline__ long long pages_of(long long len, uint32_t shift) { return (len + (1ll << shift) - 1) >> shift; }
 
 // the faults of a step, in the order in which they are reported
-enum { BAD_ROW = 1, BAD_LONG = 2, BAD_PAGE = 4 };
+enum { BAD_ROW = 1, BAD_LONG = 2 };
 
 __global__ void __launch_bounds__(PLAN_THREADS) extend_kernel(PlanArgs a) {
   extern __shared__ int4 entry[]; // per request: rows up to and with it, positions held, pages taken before it, table row
@@ -102,47 +129,58 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_kernel(PlanArgs a) {
     if (!status) at.a += g, at.b += pages_of(o + g, a.page_shift) - pages_of(o, a.page_shift);
   }
   __syncthreads();
-  const uint32_t tokens = status ? 0u : (uint32_t)total.a;
-  const uint32_t step = gridDim.x * blockDim.x, first = blockIdx.x * blockDim.x + threadIdx.x;
-  const uint32_t mask = (1u << a.page_shift) - 1;
-  for (uint32_t t = first; t < a.rows; t += step) {
-    int64_t slot = -1;
-    int32_t pos = -1, r = -1;
-    if (t < tokens) {
-      uint32_t lo = 0, hi = a.n - 1; // the first request whose rows end behind t
-      while (lo < hi) {
-        const uint32_t mid = (lo + hi) / 2;
-        if ((uint32_t)entry[mid].x > t) hi = mid;
-        else lo = mid + 1;
+  const uint32_t tokens = status ? 0u : (uint32_t)total.a, mask = (1u << a.page_shift) - 1;
+  const uint32_t step = gridDim.x * blockDim.x * ROWS_AT_ONCE;
+  for (uint32_t t0 = (blockIdx.x * blockDim.x + threadIdx.x) * ROWS_AT_ONCE; t0 < a.rows; t0 += step) {
+    int64_t slot[ROWS_AT_ONCE];
+    int32_t pos[ROWS_AT_ONCE], req[ROWS_AT_ONCE];
+    uint32_t i = t0 < tokens ? find(entry, a.n, t0) : 0;
+    const int32_t* from[ROWS_AT_ONCE]; // where a row's page is found
+#pragma unroll
+    for (uint32_t k = 0; k < ROWS_AT_ONCE; k++) {
+      const uint32_t t = t0 + k;
+      pos[k] = req[k] = -1, from[k] = nullptr;
+      if (t < tokens) {
+        while ((uint32_t)entry[i].x <= t) i++;
+        const int4 e = entry[i];
+        const uint32_t start = i ? (uint32_t)entry[i - 1].x : 0u;
+        pos[k] = e.y + (int32_t)(t - start), req[k] = e.w;
+        const uint32_t p = (uint32_t)pos[k] >> a.page_shift, had = (uint32_t)pages_of(e.y, a.page_shift);
+        from[k] = p < had ? a.table + (size_t)e.w * a.max_pages + p : a.free + (n_free - 1 - (e.z + (int32_t)(p - had)));
       }
-      const int4 e = entry[lo];
-      const uint32_t start = lo ? (uint32_t)entry[lo - 1].x : 0u;
-      pos = e.y + (int32_t)(t - start), r = e.w;
-      const uint32_t p = (uint32_t)pos >> a.page_shift, had = (uint32_t)pages_of(e.y, a.page_shift);
-      const int32_t page = p < had ? a.table[(size_t)r * a.max_pages + p] : a.free[n_free - 1 - (e.z + (int32_t)(p - had))];
-      slot = ((int64_t)page << a.page_shift) + (pos & mask);
     }
-    if (a.slot) a.slot[t] = slot;
-    if (a.position) a.position[t] = pos;
-    if (a.request) a.request[t] = r;
+#pragma unroll
+    for (uint32_t k = 0; k < ROWS_AT_ONCE; k++) {
+      const int32_t page = from[k] ? *from[k] : -1;
+      slot[k] = from[k] ? ((int64_t)page << a.page_shift) + (pos[k] & mask) : -1;
+      if (from[k] && (pos[k] & mask) == 0) a.table[(size_t)req[k] * a.max_pages + ((uint32_t)pos[k] >> a.page_shift)] = page;
+    }
+    if (t0 + ROWS_AT_ONCE <= a.rows && a.vectors) {
+      if (a.slot)
+#pragma unroll
+        for (uint32_t k = 0; k < ROWS_AT_ONCE; k += 2) *reinterpret_cast<longlong2*>(a.slot + t0 + k) = make_longlong2(slot[k], slot[k + 1]);
+      if (a.position) *reinterpret_cast<int4*>(a.position + t0) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      if (a.request) *reinterpret_cast<int4*>(a.request + t0) = make_int4(req[0], req[1], req[2], req[3]);
+    } else {
+#pragma unroll
+      for (uint32_t k = 0; k < ROWS_AT_ONCE; k++)
+        if (t0 + k < a.rows) {
+          if (a.slot) a.slot[t0 + k] = slot[k];
+          if (a.position) a.position[t0 + k] = pos[k];
+          if (a.request) a.request[t0 + k] = req[k];
+        }
+    }
   }
-  cluster_barrier(); // every CTA has read lengths, table and stack height
-  for (uint32_t i = first; i < a.n; i += step) {
+  // what the requests have now: by the CTA that arrives last, when every other one has read
+  if (!arrive_last(a.arrived)) return;
+  for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) {
     const int4 e = entry[i];
-    const uint32_t start = i ? (uint32_t)entry[i - 1].x : 0u;
-    const int32_t g = status ? 0 : e.x - (int32_t)start;
-    if (status) {
-      a.starts[i] = 0;
-      if (a.lens_out != a.lens && (uint32_t)e.w < a.requests) a.lens_out[e.w] = a.lens[e.w];
-      continue;
-    }
-    a.starts[i] = (int32_t)start;
-    const uint32_t had = (uint32_t)pages_of(e.y, a.page_shift), has = (uint32_t)pages_of((long long)e.y + g, a.page_shift);
-    int32_t* row = a.table + (size_t)e.w * a.max_pages;
-    for (uint32_t p = had; p < has; p++) row[p] = a.free[n_free - 1 - (e.z + (int32_t)(p - had))];
-    a.lens_out[e.w] = e.y + g;
+    const int32_t start = i ? entry[i - 1].x : 0;
+    a.starts[i] = status ? 0 : start;
+    if (!status) a.lens_out[e.w] = e.y + (e.x - start);
+    else if (a.lens_out != a.lens && (uint32_t)e.w < a.requests) a.lens_out[e.w] = a.lens[e.w];
   }
-  if (first == 0) {
+  if (threadIdx.x == 0) {
     a.starts[a.n] = (int32_t)tokens;
     *a.n_free_out = status ? n_free : n_free - (int32_t)total.b;
     *a.status = status;
@@ -150,19 +188,19 @@ __global__ void __launch_bounds__(PLAN_THREADS) extend_kernel(PlanArgs a) {
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) release_kernel(PlanArgs a) {
-  extern __shared__ int4 entry[]; // per request: pages held, -, pages of the requests before it, table row
+  extern __shared__ int4 entry[]; // per request: pages up to and with it, -, -, table row
   grid_wait();
   const uint32_t per = (a.n + blockDim.x - 1) / blockDim.x, i0 = threadIdx.x * per, i1 = min(a.n, i0 + per);
   const int32_t n_free = *a.n_free;
-  int bad = (uint32_t)n_free > a.n_pages ? BAD_ROW : 0;
+  int bad = (uint32_t)n_free > a.n_pages;
   Pair mine{0, 0};
   for (uint32_t i = i0; i < i1; i++) {
     const int32_t r = a.req ? a.req[i] : (int32_t)i;
     long long held = 0;
-    if ((uint32_t)r >= a.requests) bad = BAD_ROW;
+    if ((uint32_t)r >= a.requests) bad = 1;
     else {
       const int32_t o = a.lens[r];
-      if (o < 0 || (long long)o > ((long long)a.max_pages << a.page_shift)) bad = BAD_ROW;
+      if (o < 0 || (long long)o > ((long long)a.max_pages << a.page_shift)) bad = 1;
       else held = pages_of(o, a.page_shift);
     }
     entry[i] = make_int4((int32_t)held, 0, 0, r);
@@ -171,64 +209,61 @@ __global__ void __launch_bounds__(PLAN_THREADS) release_kernel(PlanArgs a) {
   bad = __syncthreads_or(bad);
   Pair total;
   Pair at = scan_pair(mine, total);
-  for (uint32_t i = i0; i < i1; i++) {
-    entry[i].z = (int32_t)at.b;
-    at.b += entry[i].x;
-  }
-  int32_t status = bad ? FC_ERR_RANGE : total.b > (long long)a.n_pages - n_free ? FC_ERR_SHAPE : 0;
+  const bool room = total.b <= (long long)a.n_pages - n_free;
+  for (uint32_t i = i0; i < i1 && !bad && room; i++) entry[i].x = (int32_t)(at.b += entry[i].x);
   __syncthreads();
-  const uint32_t lane = threadIdx.x & 31, warp = (blockIdx.x * blockDim.x + threadIdx.x) >> 5, warps = gridDim.x * blockDim.x / 32;
-  // (a table entry that is no page would come back as one: looked for before anything is pushed)
-  int wrong = 0;
-  if (!status)
-    for (uint32_t i = warp; i < a.n; i += warps) {
-      const int4 e = entry[i];
-      const int32_t* row = a.table + (size_t)e.w * a.max_pages;
-      for (uint32_t p = lane; p < (uint32_t)e.x; p += 32) wrong |= (uint32_t)row[p] >= a.n_pages;
-    }
+  const uint32_t pages = bad || !room ? 0u : (uint32_t)total.b, step = gridDim.x * blockDim.x * ROWS_AT_ONCE;
+  int wrong = 0; // a table entry that is no page would come back as one
+  for (uint32_t t0 = (blockIdx.x * blockDim.x + threadIdx.x) * ROWS_AT_ONCE; t0 < pages; t0 += step) {
+    uint32_t i = find(entry, a.n, t0);
+    int32_t page[ROWS_AT_ONCE];
+#pragma unroll
+    for (uint32_t k = 0; k < ROWS_AT_ONCE; k++)
+      if (t0 + k < pages) {
+        while ((uint32_t)entry[i].x <= t0 + k) i++;
+        page[k] = a.table[(size_t)entry[i].w * a.max_pages + (t0 + k - (i ? (uint32_t)entry[i - 1].x : 0u))];
+      }
+#pragma unroll
+    for (uint32_t k = 0; k < ROWS_AT_ONCE; k++)
+      if (t0 + k < pages) wrong |= (uint32_t)page[k] >= a.n_pages, a.free[n_free + (int32_t)(t0 + k)] = page[k];
+  }
   wrong = __syncthreads_or(wrong);
-  __shared__ int any_wrong;
-  if (threadIdx.x == 0) any_wrong = 0;
-  cluster_barrier();
-  if (wrong && threadIdx.x < gridDim.x) { // one word in each CTA of the cluster
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"((uint32_t)__cvta_generic_to_shared(&any_wrong)), "r"(threadIdx.x));
-    asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(remote), "r"(1) : "memory");
+  if (gridDim.x > 1 && wrong && threadIdx.x == 0) atomicOr(a.arrived + 1, 1u);
+  if (!arrive_last(a.arrived)) return;
+  if (gridDim.x > 1) {
+    wrong = __ldcg(a.arrived + 1);
+    __syncthreads();
+    if (threadIdx.x == 0) a.arrived[1] = 0;
   }
-  cluster_barrier(); // and every CTA has read lengths, table and stack height
-  if (!status && any_wrong) status = FC_ERR_RANGE;
-  for (uint32_t i = warp; i < a.n; i += warps) {
-    const int4 e = entry[i];
-    if (status) {
-      if (lane == 0 && a.lens_out != a.lens && (uint32_t)e.w < a.requests) a.lens_out[e.w] = a.lens[e.w];
-      continue;
-    }
-    const int32_t* row = a.table + (size_t)e.w * a.max_pages;
-    for (uint32_t p = lane; p < (uint32_t)e.x; p += 32) a.free[n_free + e.z + (int32_t)p] = row[p];
-    if (lane == 0) a.lens_out[e.w] = 0;
+  const int32_t status = bad || wrong ? FC_ERR_RANGE : room ? 0 : FC_ERR_SHAPE;
+  for (uint32_t i = threadIdx.x; i < a.n; i += blockDim.x) {
+    const int32_t r = entry[i].w;
+    if (!status) a.lens_out[r] = 0;
+    else if (a.lens_out != a.lens && (uint32_t)r < a.requests) a.lens_out[r] = a.lens[r];
   }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
+  if (threadIdx.x == 0) {
     *a.n_free_out = status ? n_free : n_free + (int32_t)total.b;
     *a.status = status;
   }
 }
 
-int launch_plan(FcDevice* dev, const char* what, void (*kern)(PlanArgs), const PlanArgs& a, uint32_t work) {
-  const size_t smem = (size_t)a.n * sizeof(int4);
+// `work`: rows, or an upper bound of the pages. A CTA's prefix sums take longer the fewer threads it has, its rows the fewer
+// CTAs there are.
+int launch_plan(FcDevice* dev, const char* what, void (*kern)(PlanArgs), PlanArgs a, uint64_t work) {
   static OncePerDevice once[2];
-  if (once[kern == release_kernel].first(dev->ordinal))
-    FC_CUDA(dev, cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(PLAN_MAX * sizeof(int4))));
-  // one CTA up to a row per thread, else the whole cluster
-  const uint32_t ctas = work <= PLAN_THREADS ? 1 : PLAN_CTAS;
-  const uint32_t threads = work <= 256 && a.n <= 256 ? 256 : PLAN_THREADS;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = ctas, at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.gridDim = ctas, cfg.blockDim = threads, cfg.dynamicSmemBytes = smem, cfg.stream = dev->stream, cfg.attrs = at, cfg.numAttrs = 2;
-  FC_LAUNCH(dev, what, cudaLaunchKernelEx(&cfg, kern, a));
+  OncePerDevice& set = once[kern == release_kernel];
+  if (a.n * sizeof(int4) > (48 << 10) && set.first(dev->ordinal)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(PLAN_MAX * sizeof(int4)));
+    if (e != cudaSuccess) set.again(dev->ordinal);
+    FC_CUDA(dev, e);
+  }
+  const uint32_t threads = a.n > 1024 ? PLAN_THREADS : 256;
+  const uint64_t wanted = (work + threads * ROWS_AT_ONCE - 1) / (threads * ROWS_AT_ONCE), most = dev->prop.multiProcessorCount;
+  const uint32_t ctas = wanted < 1 ? 1 : wanted < most ? (uint32_t)wanted : (uint32_t)most;
+  void* p = nullptr;
+  if (ctas > 1) FC_TRY(serving_scratch(dev, &dev->plan, 256, 256, &p));
+  a.arrived = static_cast<uint32_t*>(p);
+  FC_LAUNCH(dev, what, launch_on(dev, true, kern, dim3(ctas), dim3(threads), a.n * sizeof(int4), a));
   return FC_OK;
 }
 
@@ -296,7 +331,8 @@ FC_API int fc_paged_extend_dev(FcDevice* dev, const FcPagedCache* c, const int32
   if ((n && !grow) || !starts) return fc_fail(dev, FC_ERR_ARG, "fc_paged_extend_dev: grow or starts is NULL");
   if (rows > (uint32_t)INT_MAX) return fc_fail(dev, FC_ERR_SHAPE, "%u rows in a step", rows);
   a.grow = grow, a.rows = rows, a.starts = starts, a.slot = slot, a.position = position, a.request = request;
-  return launch_plan(dev, "paged_extend", extend_kernel, a, rows > n ? rows : n);
+  a.vectors = aligned_to(slot, 16) && aligned_to(position, 16) && aligned_to(request, 16);
+  return launch_plan(dev, "paged_extend", extend_kernel, a, rows);
 }
 
 FC_API int fc_paged_release_dev(FcDevice* dev, const FcPagedCache* c, const int32_t* requests, uint32_t n, int32_t* lens_out,
@@ -305,5 +341,5 @@ FC_API int fc_paged_release_dev(FcDevice* dev, const FcPagedCache* c, const int3
   cudaSetDevice(dev->ordinal);
   PlanArgs a = {};
   FC_TRY(plan_args(dev, c, requests, n, lens_out, n_free_out, status, &a));
-  return launch_plan(dev, "paged_release", release_kernel, a, n * 32);
+  return launch_plan(dev, "paged_release", release_kernel, a, std::min<uint64_t>((uint64_t)n * c->max_pages, c->n_pages));
 }

@@ -195,7 +195,7 @@ FC_API int fc_device_close(FcDevice* dev) {
   if (dev->workspaces) cudaMemPoolDestroy(dev->workspaces);
   if (dev->pinned) cudaFreeHost(dev->pinned);
   if (dev->d_flag) cudaFree(dev->d_flag);
-  for (void* p : {dev->attend.ws.p, dev->logprobs.ws.p})
+  for (void* p : {dev->attend.ws.p, dev->logprobs.ws.p, dev->plan.ws.p})
     if (p) cudaFree(p);
   for (auto& s : dev->spans) {
     cudaEventDestroy(s.t0);

@@ -62,12 +62,13 @@ def _at(dev: Device, name: str, n: int, entries: int, where: int):
 
 def _rows(dev: Device, t, name: str):
     """(address, kind, stride) of a two-dimensional device tensor whose rows are contiguous."""
-    if t.dim() != 2 or t.get_device() != dev.ordinal or not t.is_cuda:
+    stride = t.stride()
+    if len(stride) != 2 or t.get_device() != dev.ordinal:
         raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be rows on cuda:{dev.ordinal}")
-    stride, step = t.stride()
-    if step != 1 and t.shape[1] > 1:
+    if stride[1] != 1 and t.shape[1] > 1:
         raise CudaError(_ffi.FC_ERR_ARG, f"the elements of {name}'s rows must lie side by side")
-    return t.data_ptr(), _kind(t), stride
+    kind = _KINDS.get(t.dtype)
+    return t.data_ptr(), _kind(t) if kind is None else kind, stride[0]
 
 
 class _Buffers:
@@ -161,6 +162,7 @@ class PagedCache:
 
     def __init__(self, dev: Device, page: int, table=None, lens=None, free=None, n_free=None, layers=()):
         self.dev, self._lib, self.page = dev, _ffi.load(), page
+        self._append, self._attend = self._lib.fc_paged_append_dev, self._lib.fc_paged_attend_dev
         self.table, self.lens, self.free, self.n_free, self.layers = table, lens, free, n_free, list(layers)
         shapes = {(tuple(t.shape), str(t.dtype)) for kv in self.layers for t in kv}
         _need(len(shapes) <= 1, _ffi.FC_ERR_SHAPE, "every layer's k and v must have one shape and type")
@@ -226,7 +228,7 @@ class PagedCache:
             raise CudaError(_ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {hd} beside {2 * kv}")
         if q_kind != kind or q_out.shape != (rows, heads * hd):
             raise CudaError(_ffi.FC_ERR_SHAPE, f"q_out must be {rows} x {heads * hd} of qkv's type")
-        dev.check(self._lib.fc_paged_append_dev(dev.handle, self._refs[layer], rotary._ref if rotary is not None else None, at, kind, stride, rows,
+        dev.check(self._append(dev.handle, self._refs[layer], rotary._ref if rotary is not None else None, at, kind, stride, rows,
                                                 heads, step._ptr(dev, "slot", rows), step._ptr(dev, "position", rows), q_at, q_stride))
 
     def attend(self, layer: int, q, step: Step, out, scale: float = 0.0):
@@ -239,7 +241,7 @@ class PagedCache:
             raise CudaError(_ffi.FC_ERR_SHAPE, f"rows of {width} elements hold no whole heads of {view.head_dim}")
         if out_kind != kind or out.shape != q.shape:
             raise CudaError(_ffi.FC_ERR_SHAPE, "the result must have q's shape and type")
-        dev.check(self._lib.fc_paged_attend_dev(dev.handle, self._refs[layer], at, kind, stride, rows, width // view.head_dim,
+        dev.check(self._attend(dev.handle, self._refs[layer], at, kind, stride, rows, width // view.head_dim,
                                                 step._ptr(dev, "request", rows), step._ptr(dev, "position", rows), scale, out_at, out_stride))
 
     def _view(self, layer: int):

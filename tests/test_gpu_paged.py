@@ -250,8 +250,8 @@ def test_append_strides_and_alignments(dev, kw, act, neox):
 @pytest.mark.parametrize("heads,kv,hd,rope_dim", [(12, 4, 64, 64), (32, 8, 128, 96), (3, 1, 40, 24), (64, 8, 128, 128), (6, 6, 64, 0), (56, 8, 256, 256), (2, 2, 64, 40)])
 @pytest.mark.parametrize("neox", [False, True])
 def test_append_many_rows(dev, act, cache, heads, kv, hd, rope_dim, neox):
-    """Rows from narrow (a few hundred bytes) to wide (tens of KB), more than there are CTAs; with rows that are no tokens."""
-    _append_case(dev, 2500 if heads * hd < 8192 else 1100, heads, kv, hd, rope_dim, neox, act, cache, 16, seed=7, pad=8 if heads == 12 else 0, q_pad=16 if heads == 6 else 0)
+    """Rows from narrow (a few hundred bytes) to wide (tens of KB), 20 MB of them; with rows that are no tokens."""
+    _append_case(dev, 20_000_000 // ((heads + 2 * kv) * hd * (4 if act == "f32" else 2)), heads, kv, hd, rope_dim, neox, act, cache, 16, seed=7, pad=8 if heads == 12 else 0, q_pad=16 if heads == 6 else 0)
 
 
 # ---- attention ----------------------------------------------------------------------------------------------------------
