@@ -234,9 +234,10 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   __shared__ float sm_f[LP_WARPS], sm_ln;
   __shared__ uint32_t sm_u[LP_WARPS], sm_n, sm_ties, sm_listed, sm_last;
   __shared__ Share sm_share[LP_WARPS];
-  __shared__ float own_maxima[LP_GROUPS * LP_THREADS]; // of the row, in the end: a thread reads and writes its own column
+  __shared__ __align__(16) float own_maxima[LP_GROUPS * LP_THREADS]; // of the row, in the end
   __shared__ uint32_t sm_sets[32], listed[LP_CAND];
   __shared__ unsigned long long cand[LP_CAND];
+  if (threadIdx.x < 32) sm_sets[threadIdx.x] = 0;
   grid_wait();
   const uint32_t r = blockIdx.x / a.splits, split = blockIdx.x - r * a.splits, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Row<T> row(a, r);
@@ -263,6 +264,17 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   // next value below it, and than it. (Nothing lies below -inf and nothing compares with NaN: counted in a sweep of their own.)
   const bool sweep = has && !(xt > -INFINITY);
   const T behind = sweep ? from_f32<T>(INFINITY) : raw_target, before = has && !sweep ? next_below(raw_target) : from_f32<T>(INFINITY);
+  // What the vectors leave over is asked for here too: the logits outside them, and those equal to the target in front of it
+  // in its own vector (which is counted as if it lay behind the target).
+  float rest = 0.0f;
+  bool tie = false;
+  if (split == 0) {
+    if (tid < row.rest) rest = to_f32(row.x[row.rest_at(tid)]);
+    if (has && !sweep && tid < E && (uint32_t)target >= row.head && (uint32_t)target < row.head + row.vecs * E) {
+      const uint32_t i = row.head + ((uint32_t)target - row.head) / E * E + tid;
+      tie = i < (uint32_t)target && to_f32(row.x[i]) == xt;
+    }
+  }
   for (uint32_t g = 0; g < a.groups; g++) {
     float group_max = -INFINITY; // (of NaN or nothing: -inf, which reaches nothing that it should not)
     for (uint32_t st = 0; st < per && at - tid < v1; st++) {
@@ -313,16 +325,11 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     if (a.top) maxima[g * LP_THREADS + tid] = group_max;
   }
   if (split == 0 && tid < row.rest) {
-    const uint32_t i = row.rest_at(tid);
-    const float x = to_f32(row.x[i]);
-    if (x > own.m) move_to(x, own);
-    add(Base(own.m).of(x), own.s, own.t);
-    own.above += x > to_f32(i < (uint32_t)target ? before : behind);
+    if (rest > own.m) move_to(rest, own);
+    add(Base(own.m).of(rest), own.s, own.t);
+    own.above += rest > to_f32(row.rest_at(tid) < (uint32_t)target ? before : behind);
   }
-  if (split == 0 && has && !sweep && tid == 0 && (uint32_t)target >= row.head && (uint32_t)target < row.head + row.vecs * E) {
-    // (the target's own vector was counted as if it lay behind the target)
-    for (uint32_t i = row.head + ((uint32_t)target - row.head) / E * E; i < (uint32_t)target; i++) own.above += to_f32(row.x[i]) == xt;
-  }
+  own.above += tie;
   if (sweep)
     for (uint32_t i = split * LP_THREADS + tid; i < a.vocab; i += a.splits * LP_THREADS) {
       const float x = to_f32(row.x[i]);
@@ -332,6 +339,28 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   move_to(reduce(own.m, sm_f, larger), own);
   Share all = add_up(own, sm_share);
+  // The row's group maxima, of all shares, four neighbouring threads' to a lane and every fourth group to a warp: to shared
+  // memory, and the 32 sets of four threads' largest.
+  const uint32_t all_groups = a.splits * a.groups;
+  auto fetch = [&]() {
+    float4 m[LP_GROUPS / LP_WARPS];
+#pragma unroll
+    for (uint32_t i = 0; i < LP_GROUPS / LP_WARPS; i++) {
+      const uint32_t g = i * LP_WARPS + warp;
+      if (g >= all_groups) break;
+      float4* own_at = reinterpret_cast<float4*>(own_maxima + g * LP_THREADS) + lane;
+      m[i] = a.splits == 1 ? *own_at : __ldcg(reinterpret_cast<const float4*>(a.maxima + ((size_t)r * all_groups + g) * LP_THREADS) + lane);
+    }
+    uint32_t best = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < LP_GROUPS / LP_WARPS; i++) {
+      const uint32_t g = i * LP_WARPS + warp;
+      if (g >= all_groups) break;
+      best = max(best, max(max(order_of(m[i].x), order_of(m[i].y)), max(order_of(m[i].z), order_of(m[i].w))));
+      if (a.splits > 1) *(reinterpret_cast<float4*>(own_maxima + g * LP_THREADS) + lane) = m[i];
+    }
+    atomicMax(&sm_sets[lane], best);
+  };
   if (a.splits > 1) {
     if (tid == 0) a.shares[blockIdx.x] = all;
     __syncthreads();
@@ -343,23 +372,15 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     __syncthreads();
     if (!sm_last) return;
     if (tid == 0) a.arrived[r] = 0; // for the next call
-    if (a.top) {
-      const float* row_maxima = a.maxima + (size_t)r * (a.splits * a.groups) * LP_THREADS + tid;
-#pragma unroll 8
-      for (uint32_t i = 0; i < a.splits * a.groups; i++) own_maxima[i * LP_THREADS + tid] = __ldcg(row_maxima + i * LP_THREADS);
-    }
-    const Share* shares = a.shares + (size_t)r * a.splits;
-    Share mine{-INFINITY, 0.0f, 0.0f, 0u};
-    for (uint32_t i = tid; i < a.splits; i += LP_THREADS) {
-      const float4 raw = __ldcg(reinterpret_cast<const float4*>(shares + i));
-      Share one{raw.x, raw.y, raw.z, __float_as_uint(raw.w)};
-      const float high = fmaxf(mine.m, one.m);
-      move_to(high, mine), move_to(high, one);
-      mine.s += one.s, mine.t += one.t, mine.above += one.above;
-    }
-    const float top = reduce(mine.m, sm_f, larger);
-    move_to(top, mine);
-    all = add_up(mine, sm_share); // (the barriers since the first use of sm_share lie behind everyone's reads)
+    // every warp joins the shares for itself, a lane each; the slots' loads are under way meanwhile
+    const float4 raw = lane < a.splits ? __ldcg(reinterpret_cast<const float4*>(a.shares + (size_t)r * a.splits + lane)) : make_float4(-INFINITY, 0.0f, 0.0f, 0.0f);
+    if (a.top) fetch();
+    all = Share{raw.x, raw.y, raw.z, __float_as_uint(raw.w)};
+    move_to(warp_reduce(all.m, larger), all);
+    auto plus = [](auto x, auto y) { return x + y; };
+    all.s = warp_reduce(all.s, plus), all.t = warp_reduce(all.t, plus), all.above = warp_reduce(all.above, plus);
+  } else if (a.top) {
+    fetch();
   }
   const float top_logit = all.m == -INFINITY ? 0.0f : all.m;
   if (tid == 0) {
@@ -381,33 +402,33 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     if (a.top_logprob) a.top_logprob[(size_t)r * a.top + k] = key ? x - top_logit - sm_ln : -INFINITY;
   };
   auto key_of = [](uint32_t order, uint32_t i) { return (unsigned long long)order << 32 | (0xffffffffu - i); };
-  // This thread's group maxima, of all shares. The CTA's threads fall into 32 sets of 4: the k-th largest of the sets' maxima
-  // bounds the k-th largest logit (about k further logits lie above it; 130 for k = 32).
-  const uint32_t all_groups = a.splits * a.groups;
-  auto maximum = [&](uint32_t i) { return order_of(own_maxima[i * LP_THREADS + tid]); };
-  uint32_t bound = order_of(all.m); // one alternative: the maximum itself
+  // The k-th largest of the sets' maxima bounds the k-th largest logit (about half as many again lie above it for k = 20, 130
+  // for k = 32). One alternative: the maximum itself.
+  uint32_t bound = order_of(all.m);
+  const uint32_t set = sm_sets[lane];
   if (a.top > 1) {
-    uint32_t best = 0;
-#pragma unroll 4
-    for (uint32_t i = 0; i < all_groups; i++) best = max(best, maximum(i));
-#pragma unroll
-    for (int o = 1; o < LP_THREADS / 32; o <<= 1) best = max(best, __shfl_xor_sync(0xffffffffu, best, o));
-    if (lane % (LP_THREADS / 32) == 0) sm_sets[tid / (LP_THREADS / 32)] = best;
-    __syncthreads();
-    const uint32_t mine = sm_sets[lane];
     uint32_t place = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < 32; j++) place += sm_sets[j] > mine || (sm_sets[j] == mine && j < lane);
-    bound = __shfl_sync(0xffffffffu, mine, __ffs(__ballot_sync(0xffffffffu, place == a.top - 1)) - 1);
+    for (uint32_t j = 0; j < 32; j++) place += sm_sets[j] > set || (sm_sets[j] == set && j < lane);
+    bound = __shfl_sync(0xffffffffu, set, __ffs(__ballot_sync(0xffffffffu, place == a.top - 1)) - 1);
   }
-  // a share's groups all have as many steps; a group is listed as (share's group) * LP_THREADS + thread
+  // The groups that reach it, as (group of the row) * LP_THREADS + thread: the warps take the sets that do in turn, a lane a
+  // group of the set's four threads. (A share's groups all have as many steps.)
+  static_assert(LP_GROUPS <= 32 && LP_THREADS == 128, "a lane per group, sets of four threads");
   auto list = [&](bool equal_too) {
-#pragma unroll 4
-    for (uint32_t i = 0; i < all_groups; i++) {
-      const uint32_t o = maximum(i);
-      if (o > bound || (o == bound && equal_too)) {
-        const uint32_t p = atomicAdd(&sm_listed, 1u);
-        if (p < LP_CAND) listed[p] = i * LP_THREADS + tid;
+    uint32_t turn = 0;
+    for (uint32_t reach = __ballot_sync(0xffffffffu, set > bound || (set == bound && equal_too)); reach; reach &= reach - 1) {
+      if (turn++ % LP_WARPS != warp || lane >= all_groups) continue;
+      const uint32_t s = __ffs(reach) - 1;
+      const float4 m = *(reinterpret_cast<const float4*>(own_maxima + lane * LP_THREADS) + s);
+      const float x[4] = {m.x, m.y, m.z, m.w};
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) {
+        const uint32_t o = order_of(x[j]);
+        if (o > bound || (o == bound && equal_too)) {
+          const uint32_t p = atomicAdd(&sm_listed, 1u);
+          if (p < LP_CAND) listed[p] = lane * LP_THREADS + 4 * s + j;
+        }
       }
     }
     __syncthreads();
@@ -423,20 +444,32 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     list(equal_too);
     if (sm_listed <= LP_CAND) {
       const uint32_t vecs = per * VECS, total = sm_listed * vecs;
-#pragma unroll 2
-      for (uint32_t j = tid; j < total; j += LP_THREADS) {
-        const uint32_t entry = listed[j / vecs], i = entry / LP_THREADS, s = i / a.groups, g = i - s * a.groups;
-        const uint32_t at = share_at(s) + (g * per * VECS + j % vecs) * LP_THREADS + entry % LP_THREADS;
-        if (at >= share_at(s + 1)) continue;
-        const uint4 v = __ldg(row.vec(at));
-        if (order_of(Vec<T>::high(v)) < bound) continue;
-        float x[E];
-        Vec<T>::unpack(v, x);
+#pragma unroll 1
+      for (uint32_t j0 = tid; j0 < total; j0 += 4 * LP_THREADS) { // (four loads in flight)
+        uint4 v[4];
+        uint32_t at[4];
 #pragma unroll
-        for (int e = 0; e < E; e++) offer(x[e], row.head + at * E + e, equal_too);
+        for (uint32_t q = 0; q < 4; q++) {
+          const uint32_t j = j0 + q * LP_THREADS;
+          at[q] = 0xffffffffu;
+          if (j >= total) continue;
+          const uint32_t entry = listed[j / vecs], i = entry / LP_THREADS, s = i / a.groups, g = i - s * a.groups;
+          const uint32_t where = share_at(s) + (g * per * VECS + j % vecs) * LP_THREADS + entry % LP_THREADS;
+          if (where < share_at(s + 1)) v[q] = __ldg(row.vec(where)), at[q] = where;
+        }
+#pragma unroll 1
+        for (uint32_t q = 0; q < 4; q++) {
+          const uint4 now = q == 0 ? v[0] : q == 1 ? v[1] : q == 2 ? v[2] : v[3];
+          const uint32_t where = q == 0 ? at[0] : q == 1 ? at[1] : q == 2 ? at[2] : at[3];
+          if (where == 0xffffffffu || order_of(Vec<T>::high(now)) < bound) continue;
+          float x[E];
+          Vec<T>::unpack(now, x);
+#pragma unroll
+          for (int e = 0; e < E; e++) offer(x[e], row.head + where * E + e, equal_too);
+        }
       }
     }
-    if (tid < row.rest) offer(to_f32(row.x[row.rest_at(tid)]), row.rest_at(tid), equal_too);
+    if (tid < row.rest) offer(split == 0 ? rest : to_f32(row.x[row.rest_at(tid)]), row.rest_at(tid), equal_too);
     __syncthreads();
     const bool fits = sm_listed <= LP_CAND && sm_n + sm_ties <= LP_CAND;
     __syncthreads();
