@@ -2,6 +2,7 @@
 // checks of a cache's view.
 #pragma once
 #include "common.cuh"
+#include "tc_ptx.cuh"
 
 __device__ __forceinline__ float to_f32(float v) { return v; }
 __device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
@@ -19,6 +20,19 @@ __device__ __forceinline__ __half from_f32<__half>(float v) {
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
   return __float2bfloat16_rn(v);
+}
+
+// Waits for a phase of an mbarrier, for two seconds at most: false when it gave up. A parity only tells a phase from its
+// neighbours, so whoever waits has to meet every phase of the barrier in order.
+__device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
+  if (tc::mbar_try_wait(bar, parity)) return true;
+  unsigned long long t0, t;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t0));
+  do {
+    if (tc::mbar_try_wait_for(bar, parity, 1000)) return true;
+    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
+  } while (t - t0 < 2000000000ull);
+  return tc::mbar_try_wait(bar, parity);
 }
 
 static inline bool paged_kind(int kind) { return kind == FC_F32 || kind == FC_F16 || kind == FC_BF16; }

@@ -15,7 +15,6 @@
 #include <vector>
 
 #include "paged.cuh"
-#include "tc_ptx.cuh"
 
 namespace {
 
@@ -218,7 +217,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) append_rows_kernel(Appe
       const int64_t sl = __shfl_sync(0xffffffffu, slot, i);
       if (lane == 0) {
         RowStage& st = stage_of[stage];
-        if (alive && r - begin >= stages && !tc::mbar_wait(&st.empty, phase ^ 1)) {
+        if (alive && r - begin >= stages && !wait_phase(&st.empty, phase ^ 1)) {
           alive = false;
           atomicExch(a.err_flag, 1);
         }
@@ -243,7 +242,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) append_rows_kernel(Appe
     for (uint32_t i = 0; lane == 0 && i < min(end - begin, stages); i++) {
       if (stage == 0) stage = stages, phase ^= 1;
       stage--;
-      if (!tc::mbar_wait(&stage_of[stage].full, phase)) atomicExch(a.err_flag, 2);
+      if (!wait_phase(&stage_of[stage].full, phase)) atomicExch(a.err_flag, 2);
     }
     return;
   }
@@ -252,7 +251,7 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) append_rows_kernel(Appe
     if (++stage == stages) stage = 0, phase ^= 1;
     if (now != warp) continue; // (a warp per stage, so that it meets every phase of its barriers in order; fewer stages leave warps idle)
     RowStage& st = stage_of[now];
-    if (alive && !tc::mbar_wait(&st.full, ph)) {
+    if (alive && !wait_phase(&st.full, ph)) {
       alive = false; // (reported; the results are wrong, the barriers stay whole)
       if (lane == 0) atomicExch(a.err_flag, 3);
     }

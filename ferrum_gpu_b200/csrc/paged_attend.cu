@@ -28,7 +28,6 @@
 #include <type_traits>
 
 #include "paged.cuh"
-#include "tc_ptx.cuh"
 #include "tensor_map.cuh"
 
 namespace {
@@ -43,6 +42,10 @@ struct AttendArgs {
   const int32_t *request, *position, *table;
   uint64_t q_stride, out_stride;
   uint32_t rows, heads, kv_heads, group, blocks, hd, requests, max_pages, n_pages, page_shift; // blocks: of 8 heads, per kv head
+  // where a tile's rows lie in shared memory: page after page, `span` bytes each, a page's rows of the first 128 bytes, then, `block`
+  // bytes on, those of the next; in one copy per page (`merged`) or one per page and block
+  uint32_t span, block;
+  bool merged;
   int act;
   float scale; // times log2 e
   float* parts;
@@ -104,8 +107,8 @@ __device__ __forceinline__ uint4 lds16(uint32_t at) {
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
   return v;
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(dst),
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, uint64_t* bar, int32_t x, int32_t y, int32_t z) {
+  asm volatile("cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, 0, %5}], [%2];" ::"r"(dst),
                "l"(tmap), "r"(tc::smem_u32(bar)), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
@@ -155,7 +158,7 @@ struct Shape {
   static constexpr int SHARE = TP / PS, GROUPS = WARPS / SHARE;          // warps that share a tile; groups that take tiles in turn
   static constexpr uint32_t HALF = TP * BOXES * 128, STAGE = 2 * HALF;   // bytes of k (or v), of both
   static constexpr int CTAS = 2;                                         // resident on an SM
-  static constexpr int STAGES = HDP == 256 ? 5 : HDP == 64 && !F32 ? 6 : 3;
+  static constexpr int STAGES = HDP == 256 ? 4 : HDP == 64 && !F32 ? 6 : 3;
   static constexpr int Q_TERMS = F32 ? 2 : 3;
   static constexpr uint32_t Q_BYTES = HDP / (4 * E) * Q_TERMS * 32 * 16, JOIN_BYTES = 2 * ROWS8 * HDP * 4, DONE_BYTES = ROWS8 * HDP * 4;
   static constexpr uint32_t Q_OR_JOIN = Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES;
@@ -281,7 +284,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
       const uint32_t boxes = (here + (1u << box_shift) - 1) >> box_shift; // pages with positions of the tile
       const uint32_t ok0 = __ballot_sync(0xffffffffu, lane >= boxes || page0 < a.n_pages);
       const uint32_t ok1 = __ballot_sync(0xffffffffu, lane + 32 >= boxes || page1 < a.n_pages);
-      if (alive && n >= STAGES && !tc::mbar_wait(&empty[stage], phase ^ 1)) {
+      if (alive && n >= STAGES && !wait_phase(&empty[stage], phase ^ 1)) {
         alive = false;
         if (lane == 0) atomicExch(a.err_flag, 1);
       }
@@ -298,11 +301,16 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         if (i < boxes) {
           const uint32_t p = w.tile * TP + (i << box_shift), page = half ? page1 : page0;
           const int32_t y = (int32_t)((kvh << a.page_shift) + (p & mask)), z = page < a.n_pages ? (int32_t)page : 0; // (a page that is none: masked later)
-          const uint32_t dst = stages + stage * S::STAGE + (i << box_shift) * 128;
+          const uint32_t dst = stages + stage * S::STAGE + i * a.span;
+          if (a.merged) {
+            tma_load_4d(dst, &map_k, &full[stage], 0, y, z);
+            tma_load_4d(dst + S::HALF, &map_v, &full[stage], 0, y, z);
+          } else {
 #pragma unroll
-          for (int b = 0; b < S::BOXES; b++) {
-            tma_load_3d(dst + b * TP * 128, &map_k, &full[stage], b * (128 / (int)sizeof(C)), y, z);
-            tma_load_3d(dst + S::HALF + b * TP * 128, &map_v, &full[stage], b * (128 / (int)sizeof(C)), y, z);
+            for (int b = 0; b < S::BOXES; b++) {
+              tma_load_4d(dst + b * a.block, &map_k, &full[stage], b * (128 / (int)sizeof(C)), y, z);
+              tma_load_4d(dst + S::HALF + b * a.block, &map_v, &full[stage], b * (128 / (int)sizeof(C)), y, z);
+            }
           }
         }
       }
@@ -313,7 +321,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     for (uint32_t i = 0; i < min(n, (uint32_t)STAGES); i++) {
       if (stage == 0) stage = STAGES, phase ^= 1;
       stage--;
-      if (!tc::mbar_wait(&full[stage], phase) && lane == 0) atomicExch(a.err_flag, 2);
+      if (!wait_phase(&full[stage], phase) && lane == 0) atomicExch(a.err_flag, 2);
     }
     return;
   }
@@ -324,13 +332,17 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     constexpr int OWN = ROWS8 * HDP / 128;
     const bool wide = (((uintptr_t)a.out | a.out_stride * (a.act == FC_F32 ? 4 : 2)) & 15) == 0;
     uint32_t n = 0, late = 0;
+    bool alive = true;
     for (; w.at < end; n++) {
       const uint32_t tile_end = min(w.tiles, w.tile + (end - w.at));
       const uint32_t kvh = w.which / a.blocks, h0 = kvh * a.group + (w.which % a.blocks) * ROWS8;
       const uint32_t heads = min((uint32_t)ROWS8, (kvh + 1) * a.group - h0);
       const bool whole = w.tile == 0 && tile_end == w.tiles;
       const uint32_t first_tile = w.row_at + w.which * w.tiles;
-      if (!tc::mbar_wait(&done_full, n & 1) && lane == 0) atomicExch(a.err_flag, 4);
+      if (alive && !wait_phase(&done_full, n & 1)) {
+        alive = false;
+        if (lane == 0) atomicExch(a.err_flag, 4);
+      }
       float4 v[OWN];
 #pragma unroll
       for (int i = 0; i < OWN; i++) v[i] = *(reinterpret_cast<const float4*>(&sm_done[0][0]) + lane + 32 * i);
@@ -373,9 +385,14 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
 
   // ---- the multiplying warps ----
   const uint32_t g = lane >> 2, t = lane & 3, sub = warp % S::SHARE, group = warp / S::SHARE;
-  // where this lane's pieces lie in a tile: row i of eight is swizzled by i
-  const uint32_t k_at = (sub * PS + spread(g)) * 128 + ((t ^ spread(g)) << 4);
-  const uint32_t v_at = S::HALF + (sub * PS + t) * 128 + ((spread(g) ^ t) << 4);
+  // where this lane's pieces lie in eight rows (row i is swizzled by i), and where this warp's eights lie in a tile
+  const uint32_t k_at = spread(g) * 128 + ((t ^ spread(g)) << 4), v_at = S::HALF + t * 128 + ((spread(g) ^ t) << 4);
+  uint32_t eight[NT];
+#pragma unroll
+  for (int n = 0; n < NT; n++) {
+    const uint32_t i = sub * PS + n * 8, rows = a.merged ? a.block / 128 : TP; // rows of a page in the tile (a power of two)
+    eight[n] = i / rows * (rows * 128 * S::BOXES) + (i & (rows - 1)) * 128;
+  }
   uint32_t stage = 0, phase = 0, turn = 0, segment = 0;
   bool alive = true;
   // q of a segment, fetched while the one before is multiplied: lane (g, t) of piece j has channels (4 j + t) E .. of head h0 + g
@@ -455,18 +472,16 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     for (uint32_t tile = w.tile; tile < tile_end; tile++) {
       const uint32_t now = stage, ph = phase;
       if (++stage == STAGES) stage = 0, phase ^= 1;
-      // Other groups' tiles are waited for too: a parity tells two neighbouring phases of a stage apart, so a warp must not come
-      // to a stage's next phase before it has seen this one end. (No stage gets two phases ahead of a warp that waits here:
-      // GROUPS <= STAGES, and the stage of its own next tile is not refilled.)
-      static_assert(S::GROUPS <= STAGES, "a warp meets every phase of every stage");
-      if (alive && !tc::mbar_wait(&full[now], ph)) {
-        alive = false; // (reported; the results are wrong, the barriers stay whole)
-        if (lane == 0) atomicExch(a.err_flag, 3);
-      }
+      // (a stage is always the same group's, so that its warps meet every phase of its barriers in order)
+      static_assert(STAGES % S::GROUPS == 0, "a stage belongs to one group");
       if (S::GROUPS > 1) {
         const bool ours = turn == group;
         turn = turn + 1 == S::GROUPS ? 0 : turn + 1;
         if (!ours) continue;
+      }
+      if (alive && !wait_phase(&full[now], ph)) {
+        alive = false; // (reported; the results are wrong, the barriers stay whole)
+        if (lane == 0) atomicExch(a.err_flag, 3);
       }
       const uint32_t p = tile * TP + sub * PS;
       if (p < w.len) {
@@ -482,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
           const uint32_t a0[4] = {hi.x, lo.x, hi.y, lo.y}, a1[4] = {hi.z, lo.z, hi.w, lo.w};
 #pragma unroll
           for (int n = 0; n < NT; n++) {
-            const uint4 k = lds16(base_at + ((k_at + j / 2 * TP * 128 + n * 1024) ^ (j & 1) * 64));
+            const uint4 k = lds16(base_at + eight[n] + j / 2 * a.block + (k_at ^ (j & 1) * 64));
             if constexpr (F32) {
               const uint32_t k0 = tf32_high(k.x), k1 = tf32_high(k.y), k2 = tf32_high(k.z), k3 = tf32_high(k.w);
               mma<C>(s[n], a0, k0, k1);
@@ -562,7 +577,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
           for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-              v[n][x] = lds16(base_at + ((v_at + c * TP * 128 + n * 1024 + x * 512) ^ x * 64));
+              v[n][x] = lds16(base_at + eight[n] + c * a.block + ((v_at + x * 512) ^ x * 64));
               // what no position holds may be NaN, and 0 * NaN is not 0
               if (!clean && !(ok >> (2 * n + x) & 1)) v[n][x] = make_uint4(0, 0, 0, 0);
             }
@@ -636,7 +651,10 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     warps_sync();
     if (warp == 0) {
       take(1);
-      if (segment && !tc::mbar_wait(&done_empty, (segment - 1) & 1) && lane == 0) atomicExch(a.err_flag, 5);
+      if (alive && segment && !wait_phase(&done_empty, (segment - 1) & 1)) {
+        alive = false;
+        if (lane == 0) atomicExch(a.err_flag, 5);
+      }
 #pragma unroll
       for (int i = 0; i < NI; i++)
 #pragma unroll
@@ -653,7 +671,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
   }
 
   // ---- the segments whose last part this CTA has written, joined by all four warps ----
-  if (!tc::mbar_wait(&all_done, 0)) {
+  if (!wait_phase(&all_done, 0)) {
     if (lane == 0) atomicExch(a.err_flag, 6);
     return; // (each warp by itself: without the verdict none of them may go on, and none waits for another)
   }
@@ -724,20 +742,22 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
 
 constexpr uint32_t MAX_CTAS_PER_SM = 2;
 
+// k or v as [page][block of 128 bytes][row of a page: head, position][element], boxes of a page's rows in a tile. `merged`: all
+// blocks of a row in one box, where head_dim is whole blocks; else a box per block, whose channels past head_dim are zeros.
 template <typename C>
-bool cache_map(CUtensorMap* map, const void* p, const FcPagedCache* c, uint32_t tile) {
-  const cuuint64_t es = sizeof(C), rows = (cuuint64_t)c->kv_heads * c->page;
-  const cuuint64_t dims[3] = {c->head_dim, rows, c->n_pages}, strides[2] = {c->head_dim * es, rows * c->head_dim * es};
-  const cuuint32_t box[3] = {(cuuint32_t)(128 / es), c->page < tile ? c->page : tile, 1}, estr[3] = {1, 1, 1};
+bool cache_map(CUtensorMap* map, const void* p, const FcPagedCache* c, uint32_t box_rows, uint32_t boxes, bool merged) {
+  const cuuint64_t es = sizeof(C), rows = (cuuint64_t)c->kv_heads * c->page, pitch = c->head_dim * es;
+  const cuuint64_t dims[4] = {merged ? 128 / es : c->head_dim, rows, merged ? pitch / 128 : 1, c->n_pages}, strides[3] = {pitch, merged ? 128 : rows * pitch, rows * pitch};
+  const cuuint32_t box[4] = {(cuuint32_t)(128 / es), box_rows, merged ? boxes : 1, 1}, estr[4] = {1, 1, 1, 1};
   const CUtensorMapDataType type = std::is_same<C, float>::value    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                    : std::is_same<C, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  return encode_fn() && encode_fn()(map, type, 3, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  return encode_fn() && encode_fn()(map, type, 4, const_cast<void*>(p), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                                     CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename C, int HDP, int TERMS>
-int launch_attend(FcDevice* dev, const FcPagedCache* c, const AttendArgs& a) {
+int launch_attend(FcDevice* dev, const FcPagedCache* c, AttendArgs a) {
   using S = Shape<C, HDP>;
   auto kern = attend_kernel<C, HDP, TERMS>;
   static OncePerDevice once;
@@ -747,7 +767,12 @@ int launch_attend(FcDevice* dev, const FcPagedCache* c, const AttendArgs& a) {
     FC_CUDA(dev, e);
   }
   CUtensorMap mk, mv;
-  if (!cache_map<C>(&mk, c->k, c, S::TP) || !cache_map<C>(&mv, c->v, c, S::TP))
+  // One copy per page where that is whole blocks and whole eights of rows (the copy engine takes some 30 cycles for an instruction
+  // and 4 for a row of it: 64 positions of 256 bytes in pages of 16 are 8 instructions instead of 16).
+  const uint32_t box_rows = c->page < S::TP ? c->page : S::TP;
+  a.merged = c->head_dim * sizeof(C) % 128 == 0 && box_rows >= 8;
+  a.block = a.merged ? box_rows * 128 : S::TP * 128, a.span = a.merged ? box_rows * 128 * S::BOXES : box_rows * 128;
+  if (!cache_map<C>(&mk, c->k, c, box_rows, S::BOXES, a.merged) || !cache_map<C>(&mv, c->v, c, box_rows, S::BOXES, a.merged))
     return fc_fail(dev, FC_ERR_DEVICE, "no tensor map for a pool of %u pages of %u x %u x %u", c->n_pages, c->kv_heads, c->page, c->head_dim);
   const uint64_t most = (uint64_t)a.rows * a.kv_heads * a.blocks * (((((uint64_t)a.max_pages << a.page_shift) + S::TP - 1) / S::TP));
   const uint64_t ctas = (uint64_t)dev->prop.multiProcessorCount * S::CTAS;
