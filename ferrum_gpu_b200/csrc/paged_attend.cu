@@ -157,8 +157,8 @@ struct Shape {
   static constexpr int PS = F32 && HDP > 64 ? 8 : 16;                    // positions of a warp's step
   static constexpr int SHARE = TP / PS, GROUPS = WARPS / SHARE;          // warps that share a tile; groups that take tiles in turn
   static constexpr uint32_t HALF = TP * BOXES * 128, STAGE = 2 * HALF;   // bytes of k (or v), of both
-  static constexpr int CTAS = 2;                                         // resident on an SM
-  static constexpr int STAGES = HDP == 256 ? 4 : HDP == 64 && !F32 ? 6 : 3;
+  static constexpr int CTAS = HDP == 256 ? 1 : 2;                                         // resident on an SM
+  static constexpr int STAGES = HDP == 256 ? 12 : HDP == 64 && !F32 ? 6 : 3;
   static constexpr int Q_TERMS = F32 ? 2 : 3;
   static constexpr uint32_t Q_BYTES = HDP / (4 * E) * Q_TERMS * 32 * 16, JOIN_BYTES = 2 * ROWS8 * HDP * 4, DONE_BYTES = ROWS8 * HDP * 4;
   static constexpr uint32_t Q_OR_JOIN = Q_BYTES > JOIN_BYTES ? Q_BYTES : JOIN_BYTES;
