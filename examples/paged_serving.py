@@ -1,0 +1,172 @@
+"""Continuous batching over a paged cache: a Llama-style model serves requests of unequal length from one pool of pages.
+
+Every turn is one step of whatever is there: prompts that enter (all their tokens at once) beside requests that decode one
+token each. `PagedCache.extend` gives the step's tokens their pages and slots, every layer appends to the cache and attends,
+`logprobs` picks the next token with its probability, entropy and alternatives, `release` gives a finished request's pages to
+the ones that wait. The products are the library's quantised weights; norms and gates are torch, on the same stream.
+
+    python examples/paged_serving.py
+"""
+from __future__ import annotations
+
+import os
+import sys
+from collections import deque
+from dataclasses import dataclass, field
+
+import numpy as np
+import torch
+
+sys.path.insert(0, os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+
+from ferrum_gpu_b200 import (Device, LogProbs, Mode, PagedCache, QKind, RopeScaling, Rotary, Step, _ffi, logprobs,  # noqa: E402
+                             upload_quantised)
+from ferrum_gpu_b200.hostmodel import Llama, LlamaConfig, random_llama, random_tokens  # noqa: E402
+
+
+class PagedLlama:
+    """A Llama-style model whose requests share the pages of one cache; `dtype` is the cache's element type."""
+
+    def __init__(self, dev: Device, model: Llama, kind: QKind, pages: int, page: int, requests: int, max_len: int, dtype=torch.float32):
+        c = self.cfg = model.cfg
+        self.dev = dev
+        self.stream = dev.torch_stream()
+
+        def weight(k, *mats):  # [k, n] matrices side by side
+            w = np.concatenate([np.asarray(m, dtype=np.float32).reshape(k, -1) for m in mats], axis=1)
+            return upload_quantised(dev, kind, w, k, w.shape[1])
+
+        with torch.cuda.stream(self.stream):
+            def vec(a):
+                return None if a is None else torch.from_numpy(np.ascontiguousarray(a, dtype=np.float32)).cuda(dev.ordinal)
+
+            self.tok = vec(model.tok).view(c.vocab, c.dim)
+            self.layers = []
+            for b in model.blocks:
+                bias = None if b.bq is None else torch.cat([vec(b.bq), vec(b.bk), vec(b.bv)])
+                self.layers.append({
+                    "attn_norm": vec(b.attn_norm), "ffn_norm": vec(b.ffn_norm), "bias": bias,
+                    "qkv": weight(c.dim, b.wq, b.wk, b.wv), "wo": weight(c.q_dim, b.wo),
+                    "gate_up": weight(c.dim, b.gate, b.up), "down": weight(c.hidden, b.down)})
+            self.out_norm, self.head = vec(model.out_norm), weight(c.dim, model.head)
+        scaling = RopeScaling(c.rope_dim, c.rope_base, c.rope_linear_factor, c.freq_factors)
+        self.rotary = Rotary.build(dev, scaling, max_len, c.rope_type == _ffi.FC_ROPE_NEOX)
+        self.cache = PagedCache.new(dev, c.layers, c.kv_heads, c.head_dim, pages, page, requests, -(-max_len // page), dtype)
+        torch.cuda.synchronize(dev.ordinal)
+
+    def _product(self, w, x):
+        y = torch.empty(x.shape[0], w.n(), device=x.device)
+        self.dev.check(_ffi.load().fc_qmatmul_dev(w.handle, x.data_ptr(), x.shape[0], y.data_ptr(), int(Mode.EXACT_F32)))
+        return y
+
+    def _norm(self, x, gain):
+        return x * torch.rsqrt((x * x).mean(dim=1, keepdim=True) + self.cfg.eps) * gain
+
+    def step(self, requests, ids, top: int = 0):
+        """The next tokens `ids[i]` (a list each) of the table rows `requests[i]`: (logits of each one's last token, LogProbs
+        with `top` alternatives of them, Step). Runs on the handle's stream and returns before it is done."""
+        c, where = self.cfg, f"cuda:{self.dev.ordinal}"
+        grow = [len(t) for t in ids]
+        with torch.cuda.stream(self.stream):
+            def ints(values):
+                return torch.tensor(values, dtype=torch.int32, device=where)
+
+            step = Step.new(self.dev, len(requests), sum(grow))
+            self.cache.extend(ints(grow), step, requests=ints(requests))
+            x = self.tok[ints([t for one in ids for t in one]).long()]
+            rows = x.shape[0]
+            q, attended = (torch.empty(rows, c.q_dim, device=where) for _ in range(2))
+            for i, layer in enumerate(self.layers):
+                qkv = self._product(layer["qkv"], self._norm(x, layer["attn_norm"]))
+                if layer["bias"] is not None:
+                    qkv += layer["bias"]
+                self.cache.append(i, qkv, step, q, rotary=self.rotary)
+                self.cache.attend(i, q, step, attended)
+                x = x + self._product(layer["wo"], attended)
+                gate, up = self._product(layer["gate_up"], self._norm(x, layer["ffn_norm"])).split(c.hidden, dim=1)
+                x = x + self._product(layer["down"], torch.nn.functional.silu(gate) * up)
+            last = x[step.starts[1:].long() - 1]
+            logits = self._product(self.head, self._norm(last, self.out_norm))
+            out = LogProbs.new(self.dev, len(requests), max(1, top))
+            logprobs(self.dev, logits, None, out)
+        return logits, out, step
+
+    def release(self, requests):
+        with torch.cuda.stream(self.stream):
+            status = torch.zeros(1, dtype=torch.int32, device=f"cuda:{self.dev.ordinal}")
+            self.cache.release(torch.tensor(requests, dtype=torch.int32, device=status.device), status)
+        return status
+
+
+@dataclass
+class Request:
+    prompt: list
+    want: int                                     # tokens to generate
+    tokens: list = field(default_factory=list)
+    notes: list = field(default_factory=list)     # (log-probability, entropy, alternatives) of each
+
+
+def serve(model: PagedLlama, requests, top: int = 3):
+    """Runs the requests to their ends, as many at once as there are table rows and pages for, in the order they came."""
+    waiting, running = deque(requests), {}
+    places = list(range(model.cache.table.shape[0]))[::-1]
+    page, steps = model.cache.page, 0
+    free = model.cache.free.numel()
+
+    def pages(r):
+        return -(-(len(r.prompt) + r.want) // page)
+
+    while waiting or running:
+        entering = []
+        while waiting and places and pages(waiting[0]) <= free:  # (what a request may come to need is set aside when it enters)
+            r, place = waiting.popleft(), places.pop()
+            free -= pages(r)
+            running[place] = r
+            entering.append(place)
+        if not running:
+            raise RuntimeError("a request needs more pages than the pool has")
+        at = list(running)
+        ids = [running[p].prompt if p in entering else running[p].tokens[-1:] for p in at]
+        _, out, step = model.step(at, ids, top)
+        model.dev.sync()
+        steps += 1
+        if int(step.status):
+            raise RuntimeError(f"the page plan was refused: status {int(step.status)}")
+        best, lp, entropy = out.top_index.tolist(), out.top_logprob.tolist(), out.entropy.tolist()
+        done = []
+        for i, p in enumerate(at):
+            r = running[p]
+            r.tokens.append(best[i][0])
+            r.notes.append((lp[i][0], entropy[i], list(zip(best[i][1:], lp[i][1:]))))
+            if len(r.tokens) >= r.want:
+                done.append(p)
+        if done:
+            status = model.release(done)
+            model.dev.sync()
+            if int(status):
+                raise RuntimeError(f"pages were not given back: status {int(status)}")
+            for p in done:
+                free += pages(running.pop(p))
+                places.append(p)
+    return steps
+
+
+def main():
+    cfg = LlamaConfig(vocab=2000, ctx=512, dim=256, heads=8, kv_heads=2, head_dim=64, layers=4, hidden=512, rope_dim=64,
+                      rope_type=_ffi.FC_ROPE_NEOX)
+    dev = Device.open(0)
+    model = PagedLlama(dev, random_llama(cfg, seed=1, std=0.1), QKind.Q8_0, pages=60, page=16, requests=6, max_len=cfg.ctx, dtype=torch.float16)
+    rng = np.random.default_rng(2)
+    requests = [Request(random_tokens(i, int(rng.integers(1, 200)), cfg.vocab).tolist(), int(rng.integers(5, 60))) for i in range(20)]
+    steps = serve(model, requests)
+    for i, r in enumerate(requests[:5]):
+        lp, entropy, others = r.notes[0]
+        print(f"request {i}: {len(r.prompt)} tokens in, {len(r.tokens)} out, first {r.tokens[0]} at log-probability {lp:.3f} "
+              f"(entropy {entropy:.3f}, next best {others[0][0]} at {others[0][1]:.3f})")
+    print(f"{len(requests)} requests, {sum(len(r.tokens) for r in requests)} tokens in {steps} steps; "
+          f"{int(model.cache.n_free)} of {model.cache.free.numel()} pages free again")
+    dev.close()
+
+
+if __name__ == "__main__":
+    main()
