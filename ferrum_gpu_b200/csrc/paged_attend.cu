@@ -60,6 +60,23 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+typedef unsigned long long f32x2;
+__device__ __forceinline__ f32x2 pack2(float x, float y) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 template <typename C>
 __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
@@ -80,10 +97,10 @@ __device__ __forceinline__ void mma<float>(float (&d)[4], const uint32_t (&a)[4]
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// x as tf32 terms: the upper 11 bits (to nearest), then the upper 11 of what is left
+// x as tf32 terms: the upper 11 bits, then the upper 11 of what is left, both to nearest
 __device__ __forceinline__ uint32_t tf32_high(uint32_t x) { return (x + 0x1000u) & 0xffffe000u; }
 __device__ __forceinline__ uint32_t tf32_low(uint32_t x, uint32_t high) {
-  return __float_as_uint(__uint_as_float(x) - __uint_as_float(high)) & 0xffffe000u;
+  return tf32_high(__float_as_uint(__uint_as_float(x) - __uint_as_float(high)));
 }
 // two values as one register of 16-bit terms, and what the terms leave of them
 template <typename C>
@@ -461,13 +478,13 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     next_segment<TP>(a, per_row, tile_end, ahead);
     if (ahead.at < end) fetch_q(ahead);
 
-    float o[NI][E][4], top = -INFINITY, sum = 0.0f; // of head g: the maximum is the lane's four's, the sum its own positions'
+    // of head g: the maximum is the lane's four's, the sum its own positions'
+    f32x2 o[NI][E];
+    float top = -INFINITY, sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < NI; i++)
 #pragma unroll
-      for (int e = 0; e < E; e++)
-#pragma unroll
-        for (int c = 0; c < 4; c++) o[i][e][c] = 0.0f;
+      for (int e = 0; e < E; e++) o[i][e] = 0;
 
     for (uint32_t tile = w.tile; tile < tile_end; tile++) {
       const uint32_t now = stage, ph = phase;
@@ -486,11 +503,11 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
       const uint32_t p = tile * TP + sub * PS;
       if (p < w.len) {
         const uint32_t base_at = stages + now * S::STAGE;
-        float s[NT][4];
+        float s[NT][4], less[NT][4]; // (less: of an f32 cache's low terms, so that the large sums are cut off half as often)
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
-          for (int c = 0; c < 4; c++) s[n][c] = 0.0f;
+          for (int c = 0; c < 4; c++) s[n][c] = less[n][c] = 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; j++) {
           const uint4 hi = sm_q[j][0][lane], lo = sm_q[j][1][lane];
@@ -502,8 +519,8 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
               const uint32_t k0 = tf32_high(k.x), k1 = tf32_high(k.y), k2 = tf32_high(k.z), k3 = tf32_high(k.w);
               mma<C>(s[n], a0, k0, k1);
               mma<C>(s[n], a1, k2, k3);
-              mma<C>(s[n], a0, tf32_low(k.x, k0), tf32_low(k.y, k1));
-              mma<C>(s[n], a1, tf32_low(k.z, k2), tf32_low(k.w, k3));
+              mma<C>(less[n], a0, tf32_low(k.x, k0), tf32_low(k.y, k1));
+              mma<C>(less[n], a1, tf32_low(k.z, k2), tf32_low(k.w, k3));
             } else {
               mma<C>(s[n], a0, k.x, k.y);
               mma<C>(s[n], a1, k.z, k.w);
@@ -536,7 +553,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         for (int n = 0; n < NT; n++)
 #pragma unroll
           for (int x = 0; x < 2; x++) {
-            const float v = (s[n][x] + s[n][x + 2]) * mul;
+            const float v = (F32 ? (s[n][x] + (s[n][x + 2] + less[n][x])) + less[n][x + 2] : s[n][x] + s[n][x + 2]) * mul;
             s[n][x] = ok >> (2 * n + x) & 1 ? v : -INFINITY;
             best = fmaxf(best, s[n][x]);
           }
@@ -545,12 +562,11 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         if (__any_sync(0xffffffffu, best > top)) {
           const float higher = fmaxf(top, best), keep = higher == -INFINITY ? 1.0f : ex2(top - higher);
           top = higher, sum *= keep;
+          const f32x2 keep2 = pack2(keep, keep);
 #pragma unroll
           for (int i = 0; i < NI; i++)
 #pragma unroll
-            for (int e = 0; e < E; e++)
-#pragma unroll
-              for (int c = 0; c < 4; c++) o[i][e][c] *= keep; // (rows g and g + 8 are one head)
+            for (int e = 0; e < E; e++) o[i][e] = mul2(o[i][e], keep2);
         }
         const float base = top == -INFINITY ? 0.0f : top - P_LIFT;
         float pr[NT][2];
@@ -581,16 +597,22 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
               // what no position holds may be NaN, and 0 * NaN is not 0
               if (!clean && !(ok >> (2 * n + x) & 1)) v[n][x] = make_uint4(0, 0, 0, 0);
             }
+          // Every step's products start from zero and are added here: the matrix unit cuts its running sums off instead of rounding
+          // them, a bias that would grow with the length (1.9e-6 after 55 steps of 16 positions). The two terms' rows, g and
+          // g + 8, are one head.
           if constexpr (F32) {
 #pragma unroll
-            for (int n = 0; n < NT; n++) {
-              const uint32_t u[4] = {v[n][0].x, v[n][0].y, v[n][0].z, v[n][0].w}, y[4] = {v[n][1].x, v[n][1].y, v[n][1].z, v[n][1].w};
+            for (int e = 0; e < E; e++) {
+              float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-              for (int e = 0; e < E; e++) {
-                const uint32_t uh = tf32_high(u[e]), yh = tf32_high(y[e]);
-                mma<C>(o[c][e], pa[n], uh, yh);
-                mma<C>(o[c][e], pa[n], tf32_low(u[e], uh), tf32_low(y[e], yh));
+              for (int n = 0; n < NT; n++) {
+                const uint32_t u = e == 0 ? v[n][0].x : e == 1 ? v[n][0].y : e == 2 ? v[n][0].z : v[n][0].w;
+                const uint32_t y = e == 0 ? v[n][1].x : e == 1 ? v[n][1].y : e == 2 ? v[n][1].z : v[n][1].w;
+                const uint32_t uh = tf32_high(u), yh = tf32_high(y);
+                mma<C>(d, pa[n], tf32_low(u, uh), tf32_low(y, yh));
+                mma<C>(d, pa[n], uh, yh);
               }
+              o[c][e] = add2(o[c][e], add2(pack2(d[0], d[1]), pack2(d[2], d[3])));
             }
           } else {
             const uint32_t u[4][4] = {{v[0][0].x, v[0][0].y, v[0][0].z, v[0][0].w}, {v[0][1].x, v[0][1].y, v[0][1].z, v[0][1].w},
@@ -599,8 +621,10 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
             for (int e = 0; e < E; e++) {
               const uint32_t pick = e & 1 ? 0x7632u : 0x5410u;
               const uint32_t b0 = __byte_perm(u[0][e / 2], u[1][e / 2], pick), b1 = __byte_perm(u[2][e / 2], u[3][e / 2], pick);
-              mma<C>(o[c][e], pa[0], b0, b1);
-              if constexpr (TERMS == 3) mma<C>(o[c][e], pb, b0, b1);
+              float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              if constexpr (TERMS == 3) mma<C>(d, pb, b0, b1);
+              mma<C>(d, pa[0], b0, b1);
+              o[c][e] = add2(o[c][e], add2(pack2(d[0], d[1]), pack2(d[2], d[3])));
             }
           }
         }
@@ -612,10 +636,11 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
     // join the four warps: 2 and 3 hand their results to 0 and 1, 1 to 0
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    float r[NI][E][2];
 #pragma unroll
     for (int i = 0; i < NI; i++)
 #pragma unroll
-      for (int e = 0; e < E; e++) o[i][e][0] += o[i][e][2], o[i][e][1] += o[i][e][3];
+      for (int e = 0; e < E; e++) unpack2(o[i][e], r[i][e][0], r[i][e][1]);
     warps_sync(); // (all have read q)
     const uint32_t ch0 = t * E; // channels (8 i + 4 x + t) E + e of head g
     auto give = [&](uint32_t buf) {
@@ -626,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         for (int x = 0; x < 2; x++)
 #pragma unroll
           for (int e = 0; e < E; e += 4)
-            *reinterpret_cast<float4*>(&sm_o[buf][g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
+            *reinterpret_cast<float4*>(&sm_o[buf][g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(r[i][e][x], r[i][e + 1][x], r[i][e + 2][x], r[i][e + 3][x]);
     };
     auto take = [&](uint32_t buf) {
       const float m = sm_m[buf][g], higher = fmaxf(top, m), base = higher == -INFINITY ? 0.0f : higher;
@@ -639,8 +664,8 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
 #pragma unroll
           for (int e = 0; e < E; e += 4) {
             const float4 v = *reinterpret_cast<const float4*>(&sm_o[buf][g][(8 * i + 4 * x) * E + ch0 + e]);
-            o[i][e][x] = fmaf(o[i][e][x], mine, v.x * theirs), o[i][e + 1][x] = fmaf(o[i][e + 1][x], mine, v.y * theirs);
-            o[i][e + 2][x] = fmaf(o[i][e + 2][x], mine, v.z * theirs), o[i][e + 3][x] = fmaf(o[i][e + 3][x], mine, v.w * theirs);
+            r[i][e][x] = fmaf(r[i][e][x], mine, v.x * theirs), r[i][e + 1][x] = fmaf(r[i][e + 1][x], mine, v.y * theirs);
+            r[i][e + 2][x] = fmaf(r[i][e + 2][x], mine, v.z * theirs), r[i][e + 3][x] = fmaf(r[i][e + 3][x], mine, v.w * theirs);
           }
     };
     if (warp >= 2) give(warp - 2);
@@ -661,7 +686,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
         for (int x = 0; x < 2; x++)
 #pragma unroll
           for (int e = 0; e < E; e += 4)
-            *reinterpret_cast<float4*>(&sm_done[g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(o[i][e][x], o[i][e + 1][x], o[i][e + 2][x], o[i][e + 3][x]);
+            *reinterpret_cast<float4*>(&sm_done[g][(8 * i + 4 * x) * E + ch0 + e]) = make_float4(r[i][e][x], r[i][e + 1][x], r[i][e + 2][x], r[i][e + 3][x]);
       if (t == 0) done_m[g] = top, done_l[g] = sum;
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(&done_full);
