@@ -18,13 +18,19 @@ import numpy as np
 from . import _ffi
 from .device import CudaError, Device
 
-_KINDS: dict = {}  # torch's element types -> FC_*, filled when the first tensor comes by: the package loads without torch
+_KINDS: dict = {}  # torch's element types -> FC_*, and ..
+_TYPES: dict = {}  # .. the other types by name: filled when the first tensor comes by (the package loads without torch)
+
+
+def _learn():
+    import torch
+    _KINDS.update({torch.float32: _ffi.FC_F32, torch.float16: _ffi.FC_F16, torch.bfloat16: _ffi.FC_BF16})
+    _TYPES.update({"int32": torch.int32, "int64": torch.int64, "float32": torch.float32})
 
 
 def _kind(t) -> int:
     if not _KINDS:
-        import torch
-        _KINDS.update({torch.float32: _ffi.FC_F32, torch.float16: _ffi.FC_F16, torch.bfloat16: _ffi.FC_BF16})
+        _learn()
     kind = _KINDS.get(t.dtype)
     if kind is None:
         raise CudaError(_ffi.FC_ERR_UNSUPPORTED, f"elements are float32, float16 or bfloat16, not {t.dtype}")
@@ -36,19 +42,24 @@ def _need(ok, code: int, message: str):
         raise CudaError(code, message)
 
 
-def _flat(t, name: str, dtype: str = "torch.int32"):
+def _flat(t, name: str, dtype: str = "int32"):
     """(address, entries, device) of a contiguous device tensor, all of it; None: nothing."""
     if t is None:
         return None, None, None
-    if not (t.is_cuda and t.is_contiguous() and str(t.dtype) == dtype):
-        raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be a contiguous {dtype} tensor on the device")
-    return t.data_ptr(), t.numel(), t.get_device()
+    if not _TYPES:
+        _learn()
+    where = t.get_device()
+    if t.dtype is not _TYPES[dtype] or where < 0 or not t.is_contiguous():
+        raise CudaError(_ffi.FC_ERR_ARG, f"{name} must be a contiguous torch.{dtype} tensor on the device")
+    return t.data_ptr(), t.numel(), where
 
 
 def _ints(dev: Device, t, name: str, n: int = 0):
     """The address of a contiguous int32 tensor of at least `n` entries on `dev`; None: NULL."""
+    if t is None:
+        return None
     at, entries, where = _flat(t, name)
-    if at is not None:
+    if where != dev.ordinal or entries < n:
         _at(dev, name, n, entries, where)
     return at
 
@@ -76,7 +87,7 @@ class _Buffers:
     _TYPES: dict = {}
 
     def __post_init__(self):
-        object.__setattr__(self, "_at", {f.name: _flat(getattr(self, f.name), f.name, self._TYPES.get(f.name, "torch.int32")) for f in fields(self)})
+        object.__setattr__(self, "_at", {f.name: _flat(getattr(self, f.name), f.name, self._TYPES.get(f.name, "int32")) for f in fields(self)})
 
     def _ptr(self, dev: Device, name: str, n: int):
         at, entries, where = self._at[name]
@@ -144,7 +155,12 @@ class Step(_Buffers):
     position: Any = None  # int32 [rows]
     request: Any = None   # int32 [rows]: the row of the page table
     status: Any = None    # int32 [1]: 0, the number of pages that are missing, or an FC_ERR_* code
-    _TYPES = {"slot": "torch.int64"}
+    _TYPES = {"slot": "int64"}
+
+    def __post_init__(self):
+        super().__post_init__()
+        rows = {self._at[name][1] for name in ("slot", "position", "request")} - {None}
+        object.__setattr__(self, "_rows", rows.pop() if len(rows) == 1 else 0 if not rows else None)
 
     @classmethod
     def new(cls, dev: Device, requests: int, rows: int) -> "Step":
@@ -162,7 +178,7 @@ class PagedCache:
 
     def __init__(self, dev: Device, page: int, table=None, lens=None, free=None, n_free=None, layers=()):
         self.dev, self._lib, self.page = dev, _ffi.load(), page
-        self._append, self._attend = self._lib.fc_paged_append_dev, self._lib.fc_paged_attend_dev
+        self._extend, self._append, self._attend = self._lib.fc_paged_extend_dev, self._lib.fc_paged_append_dev, self._lib.fc_paged_attend_dev
         self.table, self.lens, self.free, self.n_free, self.layers = table, lens, free, n_free, list(layers)
         shapes = {(tuple(t.shape), str(t.dtype)) for kv in self.layers for t in kv}
         _need(len(shapes) <= 1, _ffi.FC_ERR_SHAPE, "every layer's k and v must have one shape and type")
@@ -200,10 +216,10 @@ class PagedCache:
         """Pages, slots and positions of the step's tokens: request `requests[i]` (a row of the table; None: i) grows by
         `grow[i]` tokens. All or nothing: see `Step.status`. Lengths and stack height change in place unless others are given."""
         dev, n = self.dev, grow.numel()
-        rows = {step._at[name][1] for name in ("slot", "position", "request")} - {None}
-        _need(len(rows) <= 1, _ffi.FC_ERR_SHAPE, "slot, position and request of a step must have one length")
-        rows = rows.pop() if rows else 0
-        dev.check(self._lib.fc_paged_extend_dev(
+        rows = step._rows
+        if rows is None:
+            raise CudaError(_ffi.FC_ERR_SHAPE, "slot, position and request of a step must have one length")
+        dev.check(self._extend(
             dev.handle, self._refs[0], _ints(dev, requests, "requests", n), _ints(dev, grow, "grow"), n, rows, step._ptr(dev, "starts", n + 1),
             step._ptr(dev, "slot", rows), step._ptr(dev, "position", rows), step._ptr(dev, "request", rows),
             _ints(dev, lens_out, "lens_out", self._requests), _ints(dev, n_free_out, "n_free_out", 1), step._ptr(dev, "status", 1)))
@@ -258,7 +274,7 @@ class LogProbs(_Buffers):
     rank: Any = None         # int32 [rows]: 0 is the greedy pick; -1 where there is no target
     top_index: Any = None    # int32 [rows, top]
     top_logprob: Any = None  # f32 [rows, top]
-    _TYPES = {"logprob": "torch.float32", "entropy": "torch.float32", "top_logprob": "torch.float32"}
+    _TYPES = {"logprob": "float32", "entropy": "float32", "top_logprob": "float32"}
 
     def __post_init__(self):
         super().__post_init__()
