@@ -5,15 +5,20 @@
 // x_t - m - ln 2 log2 S, the entropy ln 2 (log2 S - T / S). Two shares (m, S, T) of a row are joined at the larger maximum:
 // S f and f (T + S delta) with delta <= 0 the difference of the maxima and f = 2^delta.
 //
-// What bounds it is the logits' bytes (16-bit rows: also instructions, about nine per logit). A row is read once, eight
-// 16-byte loads of a thread in flight; each thread keeps a running (m, S, T) and the number of logits that rank before the
+// What bounds it is the logits' bytes, and for 16-bit rows the instructions (seven per logit, of them an exponential) and the
+// way CTAs of unequal number fill the SMs. A row is read once, four 16-byte loads of a thread in flight while it works on
+// four others (a deeper ring in shared memory took as long); each thread keeps a running (m, S, T) and the number of logits that rank before the
 // target, all of it in f32 registers. For the alternatives it only writes down the maximum of every group of logits it has
 // passed. The k-th largest of the threads' largest group maxima bounds the k-th largest logit from below: only the groups
 // that reach it (k and a few) are read again, and the logits that reach it are put in order by counting, for each, those
 // before it. Many equal logits at that bound (forbidden tokens, a row of one value) are taken in index order instead.
 //
 // Few rows are cut into shares for several CTAs, so that all SMs load; the CTA of a row that arrives last joins them, in
-// the shares' order: the same bits every time.
+// the shares' order: the same bits every time. Rows that fill the SMs stay whole (1500 of 50257 in f16, with 20 alternatives:
+// 43 us whole, 52 in two shares, 58 in three: a share's end, its reductions and barriers, costs more than evenness gives).
+//
+// Measured, with target, entropy, rank and alternatives: 1 row of 32000 (f32) 7.8 us, launch, two dependent reads and the
+// join; 64 of 151936 (f32) 19.5 us, 2.0 TB/s; 1500 of 50257 (f16) 43 us, 3.5 TB/s, 54 % of a copy's rate.
 #include <type_traits>
 
 #include "paged.cuh"
@@ -105,30 +110,33 @@ struct Vec { // 16 bytes of logits
       return fmaxf(f.x, f.y);
     }
   }
-  // logits above thr; up to 128 per call (a half2 counts its halves)
+  // Logits above thr. A comparison gives all ones, -1: added up two at a time; of 16-bit pairs the low halves' count is what the
+  // sum lacks of a multiple of 2^16, and the high halves' what is left.
   template <uint32_t N>
   static __device__ __forceinline__ uint32_t count(const uint4 (&v)[N], const T (&thr)[N]) {
-    if constexpr (sizeof(T) == 4) {
-      uint32_t n = 0;
+    uint32_t n = 0;
 #pragma unroll
-      for (uint32_t i = 0; i < N; i++)
-        n += (__uint_as_float(v[i].x) > thr[i]) + (__uint_as_float(v[i].y) > thr[i]) + (__uint_as_float(v[i].z) > thr[i]) + (__uint_as_float(v[i].w) > thr[i]);
-      return n;
-    } else if constexpr (std::is_same<T, __half>::value) {
-      __half2 n = __float2half2_rn(0.0f);
+    for (uint32_t i = 0; i < N; i++) {
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
 #pragma unroll
-      for (uint32_t i = 0; i < N; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) n = __hadd2(n, __hgt2(reinterpret_cast<const __half2*>(&v[i])[j], __half2half2(thr[i])));
-      return (uint32_t)(__low2float(n) + __high2float(n));
-    } else {
-      __nv_bfloat162 n = __float2bfloat162_rn(0.0f);
-#pragma unroll
-      for (uint32_t i = 0; i < N; i++)
-#pragma unroll
-        for (int j = 0; j < 4; j++) n = __hadd2(n, __hgt2(reinterpret_cast<const __nv_bfloat162*>(&v[i])[j], __bfloat162bfloat162(thr[i])));
-      return (uint32_t)(__low2float(n) + __high2float(n));
+      for (int j = 0; j < 4; j += 2) {
+        uint32_t m0, m1;
+        if constexpr (sizeof(T) == 4) {
+          asm("set.gt.u32.f32 %0, %1, %2;" : "=r"(m0) : "f"(__uint_as_float(w[j])), "f"(thr[i]));
+          asm("set.gt.u32.f32 %0, %1, %2;" : "=r"(m1) : "f"(__uint_as_float(w[j + 1])), "f"(thr[i]));
+        } else if constexpr (std::is_same<T, __half>::value) {
+          m0 = __hgt2_mask(*reinterpret_cast<const __half2*>(&w[j]), __half2half2(thr[i]));
+          m1 = __hgt2_mask(*reinterpret_cast<const __half2*>(&w[j + 1]), __half2half2(thr[i]));
+        } else {
+          m0 = __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), __bfloat162bfloat162(thr[i]));
+          m1 = __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j + 1]), __bfloat162bfloat162(thr[i]));
+        }
+        n += m0 + m1;
+      }
     }
+    if constexpr (sizeof(T) == 4) return 0u - n;
+    const uint32_t low = (0u - n) & 0xffffu;
+    return low + (low - ((n + low) >> 16) & 0xffffu); // n = -low + 2^16 (low - high)
   }
   static __device__ __forceinline__ uint4 nothing() { // -inf everywhere
     const uint32_t w = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
@@ -156,23 +164,6 @@ __device__ __forceinline__ void add(float d, float& s, float& t) {
   d = max_nan(d, LOWEST);
   const float e = ex2(d);
   s += e, t = fmaf(e, d, t);
-}
-typedef unsigned long long f32x2;
-__device__ __forceinline__ f32x2 pack2(float x, float y) {
-  f32x2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(f32x2 v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
-  f32x2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
-  f32x2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
 }
 // The next value below x (not NaN, not -inf); x - 0 and +0 alike.
 __device__ __forceinline__ uint32_t step_down(uint32_t bits, uint32_t sign) { return (bits & ~sign) == 0 ? sign | 1 : bits & sign ? bits + 1 : bits - 1; }
@@ -249,6 +240,7 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   float* maxima = a.splits == 1 ? own_maxima : a.maxima + (size_t)blockIdx.x * a.groups * LP_THREADS;
   Share own{-INFINITY, 0.0f, 0.0f, 0u};
   uint32_t at = v0 + tid;
+  bool forbidden = false; // this thread has met a forbidden token (or a NaN)
   uint4 v[VECS], next[VECS];
   auto load = [&](uint4 (&v)[VECS], uint32_t at) {
 #pragma unroll
@@ -299,25 +291,32 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
           add(base.of(to_f32(row.x[row.head + vec * E + i % E])), own.s, own.t);
         }
       } else {
-        const f32x2 scale = pack2(LOG2E, LOG2E), down = pack2(-base.l2, -base.l2);
-        f32x2 s = 0, t = 0;
+        // A forbidden token's part of T would be 0 * inf: the first step where one turns up is done again with distances that end
+        // at LOWEST, and so are the steps behind it (an instruction less for every logit while there is none).
+        // (Single adds and multiply-adds: packed pairs spend more on moving registers together than they save.)
+        float s[2], t[2];
+        auto sums = [&](auto bounded) {
+          s[0] = s[1] = t[0] = t[1] = 0.0f;
 #pragma unroll
-        for (uint32_t i = 0; i < VECS; i++) {
-          if (now + i * LP_THREADS >= v1) break;
-          float x[E];
-          Vec<T>::unpack(v[i], x);
+          for (uint32_t i = 0; i < VECS; i++) {
+            if (now + i * LP_THREADS >= v1) break;
+            float x[E];
+            Vec<T>::unpack(v[i], x);
 #pragma unroll
-          for (int e = 0; e < E; e += 2) {
-            float d0, d1;
-            unpack2(fma2(pack2(x[e], x[e + 1]), scale, down), d0, d1);
-            d0 = max_nan(d0, LOWEST), d1 = max_nan(d1, LOWEST);
-            const f32x2 p = pack2(ex2(d0), ex2(d1));
-            s = add2(s, p), t = fma2(p, pack2(d0, d1), t);
+            for (int e = 0; e < E; e++) {
+              float d = fmaf(x[e], LOG2E, -base.l2);
+              if constexpr (decltype(bounded)::value) d = max_nan(d, LOWEST);
+              const float p = ex2(d);
+              s[e & 1] += p, t[e & 1] = fmaf(p, d, t[e & 1]);
+            }
           }
+        };
+        if (!forbidden) {
+          sums(std::false_type());
+          forbidden = !(t[0] + t[1] == t[0] + t[1]);
         }
-        float s0, s1, t0, t1;
-        unpack2(s, s0, s1), unpack2(t, t0, t1);
-        own.s += s0 + s1, own.t += t0 + t1;
+        if (forbidden) sums(std::true_type());
+        own.s += s[0] + s[1], own.t += t[0] + t[1];
       }
 #pragma unroll
       for (uint32_t i = 0; i < VECS; i++) v[i] = next[i];
