@@ -9,7 +9,11 @@
 // row): a run of N pairs of a head - one piece for neighbouring pairs, two for the half layout -, or N channels that are only
 // copied. A thread takes the same piece of H heads, so that slot, position and the tables' values are fetched once for
 // them, and has the loads of all of them in flight; the pieces of all rows are one line, so that small heads and few rows
-// fill warps too. Calls of few rows, where latency counts, take one head a thread.
+// fill warps too. Calls of few rows, where latency counts, take one head a thread. Many rows of 16 bits go through shared
+// memory instead (below).
+//
+// Measured: 6 rows of 20 heads of 64 in f32 1.6 us of the GPU, all of it latency; 8192 rows of 48 heads of 128 in bf16, three
+// quarters of a head rotated, 37.9 us, 5.4 TB/s, 83 % of a copy's rate; 4096 such rows in f32 34.8 us, 89 %.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -181,7 +185,9 @@ __global__ void __launch_bounds__(APPEND_THREADS) append_kernel(AppendArgs a) {
 
 // Many rows: a loading warp streams whole rows into shared memory with one bulk copy each, and the rows of the tables behind
 // them (position and slot are looked up 32 rows ahead, so that nothing waits for an address); each of the other warps owns a
-// stage, rotates its rows from shared memory and stores them. No load latency is left in the warps that store.
+// stage, rotates its rows from shared memory and stores them. No load latency is left in the warps that store (8192 rows of
+// 48 heads of 128 in bf16: 37.9 us; threads that load for themselves 70.5). Short rows, 2.5 KB, leave the warps at the
+// latency of their own instructions: 8192 of them 21.6 us, three times what their bytes need.
 constexpr int ROW_WARPS = 8 /* one per stage */, ROW_THREADS = ROW_WARPS * 32 + 32;
 constexpr uint64_t ROW_LEAST = 12 << 20; // bytes of rows from which on this is the faster way (1024 of 12 KB: 7.4 us and 7.6; 2048: 12.8 and 18.7)
 constexpr uint32_t ROW_STAGES = 8, ROW_SHARED = 110 << 10, ROW_CTAS = 2;
@@ -292,13 +298,13 @@ __global__ void __launch_bounds__(ROW_THREADS, ROW_CTAS) append_rows_kernel(Appe
         }
       } else if constexpr (N > 1) {
         if (turn) {
-        float cs[N / 2], sn[N / 2];
-        load_run<float, N / 2>(cos + ch / 2, cs), load_run<float, N / 2>(sin + ch / 2, sn);
+          float cs[N / 2], sn[N / 2];
+          load_run<float, N / 2>(cos + ch / 2, cs), load_run<float, N / 2>(sin + ch / 2, sn);
 #pragma unroll
-        for (int e = 0; e < N / 2; e++) {
-          const float u = x[2 * e], w = x[2 * e + 1];
-          x[2 * e] = fmaf(u, cs[e], -(w * sn[e])), x[2 * e + 1] = fmaf(u, sn[e], w * cs[e]);
-        }
+          for (int e = 0; e < N / 2; e++) {
+            const float u = x[2 * e], w = x[2 * e + 1];
+            x[2 * e] = fmaf(u, cs[e], -(w * sn[e])), x[2 * e + 1] = fmaf(u, sn[e], w * cs[e]);
+          }
         }
       }
       if (head < a.heads) {
@@ -339,21 +345,26 @@ int launch_rows(FcDevice* dev, const AppendArgs& a, uint32_t stages, uint32_t st
 
 template <typename T, typename C>
 int launch_append(FcDevice* dev, AppendArgs a, uint32_t rope_dim, bool aligned8, bool aligned4, bool aligned2) {
-  // the widest piece that pairs, tables and addresses allow (8192 rows of 48 x 128 in bf16, L2 flushed: 70 us with 8, 86 with 4, 121 with 2, 174 with 1)
-  const uint32_t whole = rope_dim == 0 ? 8 : a.neox ? a.half : rope_dim, table = a.neox ? a.half : a.half;
-  auto fits = [&](uint32_t n, bool aligned) { return aligned && whole % n == 0 && table % (a.neox ? n : n / 2) == 0; };
+  // the widest piece that pairs, tables and addresses allow
+  const uint32_t whole = rope_dim == 0 ? 8 : a.neox ? a.half : rope_dim;
+  auto fits = [&](uint32_t n, bool aligned) { return aligned && whole % n == 0 && a.half % (a.neox ? n : n / 2) == 0; };
   const uint32_t n = fits(8, aligned8) ? 8 : fits(4, aligned4) ? 4 : fits(2, aligned2) ? 2 : 1;
   a.turned = n == 1 ? a.half : (a.neox ? a.half : rope_dim) / n;
   a.per_head = div_by(a.turned + (a.hd - rope_dim) / n), a.per_v = div_by(a.hd / n);
-  const uint32_t table_bytes = a.half % 4 == 0 && aligned_to(a.cos, 16) && aligned_to(a.sin, 16) ? a.half * 4 : 0;
-  const uint32_t row_bytes = (a.heads + 2 * a.kv_heads) * a.hd * (uint32_t)sizeof(T), stage_bytes = (row_bytes + 2 * table_bytes + 127) / 128 * 128;
-  const uint32_t stages = std::min(ROW_STAGES, (ROW_SHARED - 512) / stage_bytes);
-  if (aligned_to(a.qkv, 16) && a.stride * sizeof(T) % 16 == 0 && stages >= 3 && (uint64_t)a.rows * row_bytes >= ROW_LEAST && n != 2) {
-    a.items = div_by((a.heads + a.kv_heads) * a.per_head.d + a.kv_heads * a.per_v.d);
-    return n == 8   ? launch_rows<T, C, 8>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
-           : n == 4 ? launch_rows<T, C, 4>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
-           : n == 2 ? launch_rows<T, C, 2>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
-                    : launch_rows<T, C, 1>(dev, a, stages, stage_bytes, row_bytes, table_bytes);
+  // Whole rows through shared memory where they are many, of 16 bits, and a CTA holds a few of them. Measured against threads that
+  // load for themselves: rows of 6144 elements, 8192 of them, pieces of 8 37.9 us and 70.5, of 4 53.0 and 68.8, of 1 125 and 143,
+  // but of 2 86.4 and 76.1; 8192 of 1280 elements 21.6 and 25.8. f32 rows, which have twice the bytes for the same
+  // instructions: 4096 of 6144 38.7 and 34.8, pieces of 4 45.0 and 35.8, of 1 115 and 71.6.
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t table_bytes = a.half % 4 == 0 && aligned_to(a.cos, 16) && aligned_to(a.sin, 16) ? a.half * 4 : 0;
+    const uint32_t row_bytes = (a.heads + 2 * a.kv_heads) * a.hd * (uint32_t)sizeof(T), stage_bytes = (row_bytes + 2 * table_bytes + 127) / 128 * 128;
+    const uint32_t stages = std::min(ROW_STAGES, (ROW_SHARED - 512) / stage_bytes);
+    if (aligned_to(a.qkv, 16) && a.stride * sizeof(T) % 16 == 0 && stages >= 3 && (uint64_t)a.rows * row_bytes >= ROW_LEAST && n != 2) {
+      a.items = div_by((a.heads + a.kv_heads) * a.per_head.d + a.kv_heads * a.per_v.d);
+      return n == 8   ? launch_rows<T, C, 8>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
+             : n == 4 ? launch_rows<T, C, 4>(dev, a, stages, stage_bytes, row_bytes, table_bytes)
+                      : launch_rows<T, C, 1>(dev, a, stages, stage_bytes, row_bytes, table_bytes);
+    }
   }
   // four heads a thread, unless the pieces of single heads do not even fill the SMs
   auto count = [&](uint32_t h) { return (uint64_t)((a.heads + a.kv_heads + h - 1) / h) * a.per_head.d + (uint64_t)((a.kv_heads + h - 1) / h) * a.per_v.d; };

@@ -791,6 +791,11 @@ int launch_attend(FcDevice* dev, const FcPagedCache* c, AttendArgs a) {
     if (e != cudaSuccess) once.again(dev->ordinal);
     FC_CUDA(dev, e);
   }
+  const uint64_t row_most = (((uint64_t)a.max_pages << a.page_shift) + S::TP - 1) / S::TP, per_row = (uint64_t)a.rows * a.kv_heads * a.blocks;
+  if (row_most > 0xffffffffull / per_row) // (tiles are counted in 32 bits)
+    return fc_fail(dev, FC_ERR_UNSUPPORTED, "%u rows of %u heads over page tables of %u x %u positions: more than one call holds", a.rows, a.heads,
+                   c->max_pages, c->page);
+  const uint64_t most = per_row * row_most;
   CUtensorMap mk, mv;
   // One copy per page where that is whole blocks and whole eights of rows (the copy engine takes some 30 cycles for an instruction
   // and 4 for a row of it: 64 positions of 256 bytes in pages of 16 are 8 instructions instead of 16).
@@ -799,7 +804,6 @@ int launch_attend(FcDevice* dev, const FcPagedCache* c, AttendArgs a) {
   a.block = a.merged ? box_rows * 128 : S::TP * 128, a.span = a.merged ? box_rows * 128 * S::BOXES : box_rows * 128;
   if (!cache_map<C>(&mk, c->k, c, box_rows, S::BOXES, a.merged) || !cache_map<C>(&mv, c->v, c, box_rows, S::BOXES, a.merged))
     return fc_fail(dev, FC_ERR_DEVICE, "no tensor map for a pool of %u pages of %u x %u x %u", c->n_pages, c->kv_heads, c->page, c->head_dim);
-  const uint64_t most = (uint64_t)a.rows * a.kv_heads * a.blocks * (((((uint64_t)a.max_pages << a.page_shift) + S::TP - 1) / S::TP));
   const uint64_t ctas = (uint64_t)dev->prop.multiProcessorCount * S::CTAS;
   FC_LAUNCH(dev, "paged_attend", launch_on(dev, true, kern, dim3((unsigned)(most < ctas ? most : ctas)), dim3(THREADS), S::BYTES, mk, mv, a));
   return FC_OK;
@@ -842,10 +846,6 @@ FC_API int fc_paged_attend_dev(FcDevice* dev, const FcPagedCache* c, const void*
   if (!std::isfinite(scale)) return fc_fail(dev, FC_ERR_ARG, "the scale is not finite");
   if (!request && rows > c->requests) return fc_fail(dev, FC_ERR_RANGE, "%u rows in a table of %u requests", rows, c->requests);
   if (!rows) return FC_OK;
-  const uint64_t row_most = ((uint64_t)c->max_pages * c->page + 7) / 8;
-  if ((uint64_t)rows * heads * row_most > 0xffffffffull) // (tiles are counted in 32 bits)
-    return fc_fail(dev, FC_ERR_UNSUPPORTED, "%u rows of %u heads over page tables of %u x %u positions: more than one call holds", rows, heads,
-                   c->max_pages, c->page);
   AttendArgs a = {};
   a.q = q, a.k = c->k, a.v = c->v, a.out = out, a.request = request, a.position = position, a.table = c->table;
   a.q_stride = q_stride, a.out_stride = out_stride, a.heads = heads, a.kv_heads = c->kv_heads, a.hd = c->head_dim;

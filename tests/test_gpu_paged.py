@@ -456,6 +456,27 @@ def test_a_captured_step_replays_with_new_lengths(dev):
             assert float((out[r].double().view(kv, heads // kv, hd) - want).abs().max()) < 1e-4
         assert not out[3:].any()
 
+def test_attend_table_limits(dev):
+    """A call's tiles are counted in 32 bits: wide page tables under many rows are taken as far as that goes, and refused behind it."""
+    f = torch.zeros
+    pool = f(1, 1, 256, 8, device="cuda") + 1
+    table = f(1, 1 << 20, dtype=torch.int32, device="cuda")  # 2^28 positions: 2^22 tiles of 64
+    cache = PagedCache(dev, 256, table=table, layers=[(pool, pool)])
+
+    def call(rows):
+        q, out = f(rows, 32, device="cuda"), f(rows, 32, device="cuda")
+        step = Step(position=f(rows, dtype=torch.int32, device="cuda") + 2, request=f(rows, dtype=torch.int32, device="cuda"))
+        torch.cuda.synchronize()
+        cache.attend(0, q, step, out)
+        _sync(dev)
+        return out
+
+    assert (call(1000) == 1).all()
+    with pytest.raises(CudaError, match="more than one call holds") as e:
+        call(1025)
+    assert e.value.code == _ffi.FC_ERR_UNSUPPORTED
+
+
 
 def test_results_do_not_change_from_call_to_call(dev):
     g = _gen(5)
