@@ -27,7 +27,8 @@ namespace {
 
 constexpr uint32_t TOP_MAX = 32;
 constexpr int LP_THREADS = 128, LP_WARPS = LP_THREADS / 32;
-constexpr uint32_t LP_GROUPS = 32;  // groups of a thread's logits in a row, over all its shares: their maxima are written down
+constexpr uint32_t LP_GROUPS = 32;  // groups of a thread's logits in a row, over all its shares, at most: their maxima are written down
+constexpr uint32_t LP_SHARE_GROUPS = 8; // and in a share
 constexpr uint32_t LP_CTAS = 6;     // CTAs resident on an SM
 constexpr uint32_t LP_CAND = 512;   // logits put in order by counting
 constexpr float LOG2E = 1.44269504088896340736f, LN2 = 0.69314718055994530942f;
@@ -225,8 +226,9 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   __shared__ float sm_f[LP_WARPS], sm_ln;
   __shared__ uint32_t sm_u[LP_WARPS], sm_n, sm_ties, sm_listed, sm_last;
   __shared__ Share sm_share[LP_WARPS];
-  __shared__ __align__(16) float own_maxima[LP_GROUPS * LP_THREADS]; // of the row, in the end
-  __shared__ uint32_t sm_sets[32], listed[LP_CAND];
+  __shared__ __align__(16) float own_maxima[LP_SHARE_GROUPS * LP_THREADS]; // of a row that is one share
+  __shared__ uint32_t sm_sets[32];
+  __shared__ uint2 listed[LP_CAND]; // a group's first vector, and where its share ends
   __shared__ unsigned long long cand[LP_CAND];
   if (threadIdx.x < 32) sm_sets[threadIdx.x] = 0;
   grid_wait();
@@ -338,36 +340,29 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
   auto larger = [](float x, float y) { return fmaxf(x, y); };
   move_to(reduce(own.m, sm_f, larger), own);
   Share all = add_up(own, sm_share);
-  // The row's group maxima, of all shares, four neighbouring threads' to a lane and every fourth group to a warp: to shared
-  // memory, and the 32 sets of four threads' largest.
+  // The row's group maxima, of all shares, four neighbouring threads' to a lane and every fourth group to a warp, and the 32 sets
+  // of four threads' largest.
+  constexpr uint32_t HELD = LP_GROUPS / LP_WARPS;
   const uint32_t all_groups = a.splits * a.groups;
+  float4 held[HELD];
   auto fetch = [&]() {
-    float4 m[LP_GROUPS / LP_WARPS];
 #pragma unroll
-    for (uint32_t i = 0; i < LP_GROUPS / LP_WARPS; i++) {
+    for (uint32_t i = 0; i < HELD; i++) {
       const uint32_t g = i * LP_WARPS + warp;
-      if (g >= all_groups) break;
-      float4* own_at = reinterpret_cast<float4*>(own_maxima + g * LP_THREADS) + lane;
-      m[i] = a.splits == 1 ? *own_at : __ldcg(reinterpret_cast<const float4*>(a.maxima + ((size_t)r * all_groups + g) * LP_THREADS) + lane);
+      held[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+      if (g >= all_groups) continue;
+      held[i] = a.splits == 1 ? *(reinterpret_cast<const float4*>(own_maxima + g * LP_THREADS) + lane)
+                              : __ldcg(reinterpret_cast<const float4*>(a.maxima + ((size_t)r * all_groups + g) * LP_THREADS) + lane);
     }
-    uint32_t best = 0;
+    float best = -INFINITY;
 #pragma unroll
-    for (uint32_t i = 0; i < LP_GROUPS / LP_WARPS; i++) {
-      const uint32_t g = i * LP_WARPS + warp;
-      if (g >= all_groups) break;
-      best = max(best, max(max(order_of(m[i].x), order_of(m[i].y)), max(order_of(m[i].z), order_of(m[i].w))));
-      if (a.splits > 1) *(reinterpret_cast<float4*>(own_maxima + g * LP_THREADS) + lane) = m[i];
-    }
-    atomicMax(&sm_sets[lane], best);
+    for (uint32_t i = 0; i < HELD; i++) best = fmaxf(best, fmaxf(fmaxf(held[i].x, held[i].y), fmaxf(held[i].z, held[i].w)));
+    atomicMax(&sm_sets[lane], order_of(best));
   };
   if (a.splits > 1) {
     if (tid == 0) a.shares[blockIdx.x] = all;
     __syncthreads();
-    if (tid == 0) { // (the barriers carry the fences' order to the CTA's other threads)
-      __threadfence();
-      sm_last = atomicAdd(&a.arrived[r], 1u) == a.splits - 1;
-      __threadfence();
-    }
+    if (tid == 0) sm_last = arrive_at(&a.arrived[r]) == a.splits - 1; // (the barriers carry its order to the CTA's other threads)
     __syncthreads();
     if (!sm_last) return;
     if (tid == 0) a.arrived[r] = 0; // for the next call
@@ -411,33 +406,30 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
     for (uint32_t j = 0; j < 32; j++) place += sm_sets[j] > set || (sm_sets[j] == set && j < lane);
     bound = __shfl_sync(0xffffffffu, set, __ffs(__ballot_sync(0xffffffffu, place == a.top - 1)) - 1);
   }
-  // The groups that reach it, as (group of the row) * LP_THREADS + thread: the warps take the sets that do in turn, a lane a
-  // group of the set's four threads. (A share's groups all have as many steps.)
-  static_assert(LP_GROUPS <= 32 && LP_THREADS == 128, "a lane per group, sets of four threads");
-  auto list = [&](bool equal_too) {
-    uint32_t turn = 0;
-    for (uint32_t reach = __ballot_sync(0xffffffffu, set > bound || (set == bound && equal_too)); reach; reach &= reach - 1) {
-      if (turn++ % LP_WARPS != warp || lane >= all_groups) continue;
-      const uint32_t s = __ffs(reach) - 1;
-      const float4 m = *(reinterpret_cast<const float4*>(own_maxima + lane * LP_THREADS) + s);
-      const float x[4] = {m.x, m.y, m.z, m.w};
+  // (Hits are few: a thread collects its own, reserves their places at once and writes them one by one.)
+  const float reach = value_of(bound);
+  auto list = [&](bool equal_too) { // (never for what equals a bound of -inf)
+    uint32_t hits = 0;
 #pragma unroll
-      for (uint32_t j = 0; j < 4; j++) {
-        const uint32_t o = order_of(x[j]);
-        if (o > bound || (o == bound && equal_too)) {
-          const uint32_t p = atomicAdd(&sm_listed, 1u);
-          if (p < LP_CAND) listed[p] = lane * LP_THREADS + 4 * s + j;
-        }
+    for (uint32_t i = 0; i < HELD; i++) {
+      const float x[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
+#pragma unroll
+      for (uint32_t j = 0; j < 4; j++) hits |= (uint32_t)(x[j] > reach || (x[j] == reach && equal_too)) << (4 * i + j);
+    }
+    if (hits) {
+      uint32_t p = atomicAdd(&sm_listed, (uint32_t)__popc(hits));
+      for (; hits; hits &= hits - 1, p++) {
+        const uint32_t bit = __ffs(hits) - 1, i = bit / 4 * LP_WARPS + warp, s = i / a.groups, g = i - s * a.groups;
+        if (p < LP_CAND) listed[p] = make_uint2(share_at(s) + g * per * STEP + 4 * lane + bit % 4, share_at(s + 1));
       }
     }
     __syncthreads();
   };
   // The logits above the bound, from the front of the list, and those equal to it, from its end.
   auto offer = [&](float x, uint32_t i, bool equal_too) {
-    const uint32_t o = order_of(x);
-    if (!o || o < bound || (o == bound && !equal_too)) return;
-    const uint32_t p = atomicAdd(o > bound ? &sm_n : &sm_ties, 1u);
-    if (p < LP_CAND) cand[o > bound ? p : LP_CAND - 1 - p] = key_of(o, i);
+    if (!(x > reach || (x == reach && equal_too))) return;
+    const uint32_t p = atomicAdd(x > reach ? &sm_n : &sm_ties, 1u);
+    if (p < LP_CAND) cand[x > reach ? p : LP_CAND - 1 - p] = key_of(order_of(x), i);
   };
   auto gather = [&](bool equal_too) {
     list(equal_too);
@@ -449,22 +441,20 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
         uint32_t at[4];
 #pragma unroll
         for (uint32_t q = 0; q < 4; q++) {
-          const uint32_t j = j0 + q * LP_THREADS;
-          at[q] = 0xffffffffu;
+          const uint32_t j = j0 + q * LP_THREADS, entry = j / vecs;
+          v[q] = Vec<T>::nothing(), at[q] = 0;
           if (j >= total) continue;
-          const uint32_t entry = listed[j / vecs], i = entry / LP_THREADS, s = i / a.groups, g = i - s * a.groups;
-          const uint32_t where = share_at(s) + (g * per * VECS + j % vecs) * LP_THREADS + entry % LP_THREADS;
-          if (where < share_at(s + 1)) v[q] = __ldg(row.vec(where)), at[q] = where;
+          const uint2 from = listed[entry];
+          at[q] = from.x + (j - entry * vecs) * LP_THREADS;
+          if (at[q] < from.y) v[q] = __ldg(row.vec(at[q]));
         }
-#pragma unroll 1
-        for (uint32_t q = 0; q < 4; q++) {
-          const uint4 now = q == 0 ? v[0] : q == 1 ? v[1] : q == 2 ? v[2] : v[3];
-          const uint32_t where = q == 0 ? at[0] : q == 1 ? at[1] : q == 2 ? at[2] : at[3];
-          if (where == 0xffffffffu || order_of(Vec<T>::high(now)) < bound) continue;
-          float x[E];
-          Vec<T>::unpack(now, x);
 #pragma unroll
-          for (int e = 0; e < E; e++) offer(x[e], row.head + where * E + e, equal_too);
+        for (uint32_t q = 0; q < 4; q++) {
+          const float high = Vec<T>::high(v[q]);
+          if (!(high >= reach) || high == -INFINITY) continue;
+          const uint32_t first = row.head + at[q] * E;
+#pragma unroll 1
+          for (uint32_t e = 0; e < E; e++) offer(to_f32(row.x[first + e]), first + e, equal_too);
         }
       }
     }
@@ -544,16 +534,16 @@ FC_API int fc_logprobs_dev(FcDevice* dev, const void* logits, int kind, uint32_t
   if (rows && !aligned_to(logits, paged_bytes(kind))) return fc_fail(dev, FC_ERR_ARG, "logits must be aligned to their elements");
   if (rows > (1u << 30)) return fc_fail(dev, FC_ERR_SHAPE, "%u rows", rows);
   if (!rows) return FC_OK;
-  LogprobArgs a{logits, stride, vocab, top_index || top_logprob ? top : 0u, 1u, 8u, targets, logprob, entropy, rank, top_index, top_logprob, nullptr, nullptr, nullptr};
+  LogprobArgs a{logits, stride, vocab, top_index || top_logprob ? top : 0u, 1u, LP_SHARE_GROUPS, targets, logprob, entropy, rank, top_index, top_logprob, nullptr, nullptr, nullptr};
   // shares of a row: as many as there are SMs' CTAs left for it, each of whole steps
   const uint32_t ctas = (uint32_t)dev->prop.multiProcessorCount * LP_CTAS;
   const uint64_t steps = ((uint64_t)vocab * paged_bytes(kind) + LP_THREADS * 64 - 1) / (LP_THREADS * 64);
   if (rows < ctas && steps > 1) a.splits = (uint32_t)min(min(steps, (uint64_t)(ctas / rows)), (uint64_t)LP_GROUPS);
   if (a.splits > 1) {
-    a.groups = min(8u, LP_GROUPS / a.splits);
+    a.groups = min(LP_SHARE_GROUPS, LP_GROUPS / a.splits);
     const size_t words = ((size_t)ctas * 4 + 255) / 256 * 256, shares = ((size_t)ctas * sizeof(Share) + 255) / 256 * 256;
     void* p;
-    FC_TRY(serving_scratch(dev, &dev->logprobs, words, words + shares + (size_t)ctas * 8 * LP_THREADS * 4, &p));
+    FC_TRY(serving_scratch(dev, &dev->logprobs, words, words + shares + (size_t)ctas * LP_SHARE_GROUPS * LP_THREADS * 4, &p));
     a.arrived = static_cast<uint32_t*>(p);
     a.shares = reinterpret_cast<Share*>(static_cast<char*>(p) + words);
     a.maxima = reinterpret_cast<float*>(static_cast<char*>(p) + words + shares);

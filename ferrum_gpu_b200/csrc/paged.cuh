@@ -35,6 +35,15 @@ __device__ __forceinline__ bool wait_phase(uint64_t* bar, uint32_t parity) {
   return tc::mbar_try_wait(bar, parity);
 }
 
+// Counts an arrival, after whatever this thread, and through a barrier its warp or CTA, has written; what those counted before
+// had written is visible behind it, through a barrier to the others too. (One instruction: a relaxed one between two fences
+// took 0.4 us longer.)
+__device__ __forceinline__ uint32_t arrive_at(uint32_t* counter) {
+  uint32_t before;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(counter) : "memory");
+  return before;
+}
+
 static inline bool paged_kind(int kind) { return kind == FC_F32 || kind == FC_F16 || kind == FC_BF16; }
 static inline size_t paged_bytes(int kind) { return kind == FC_F32 ? 4 : 2; }
 static inline bool aligned_to(const void* p, size_t bytes) { return ((uintptr_t)p & (bytes - 1)) == 0; }

@@ -381,14 +381,12 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
 #pragma unroll
         for (int i = 0; i < OWN; i++) *(reinterpret_cast<float4*>(part + 2 * ROWS8) + lane + 32 * i) = v[i];
         __syncwarp();
-        if (lane == 0) { // (the warp's barriers and the one that ends this loop carry the fences' order to the others)
+        if (lane == 0) { // (the warp's barriers and the one that ends this loop carry its order to the others)
           const uint32_t c0 = owner_of(first_tile), c1 = owner_of(first_tile + w.tiles - 1);
-          __threadfence();
-          if (atomicAdd(&a.arrived[c0], 1u) == c1 - c0) {
+          if (arrive_at(&a.arrived[c0]) == c1 - c0) {
             a.arrived[c0] = 0; // for the next call
             sm_late[late++] = {first_tile, w.tiles, w.r, h0, heads};
           }
-          __threadfence();
         }
       }
       next_segment<TP>(a, per_row, tile_end, w);

@@ -39,10 +39,8 @@ __device__ __forceinline__ bool arrive_last(uint32_t* arrived) {
   __syncthreads();
   if (gridDim.x == 1) return true;
   if (threadIdx.x == 0) {
-    __threadfence();
-    last = atomicAdd(arrived, 1u) == gridDim.x - 1;
+    last = arrive_at(arrived) == gridDim.x - 1;
     if (last) *arrived = 0; // for the next call
-    __threadfence();
   }
   __syncthreads();
   return last;
