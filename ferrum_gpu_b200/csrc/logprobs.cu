@@ -448,13 +448,17 @@ __global__ void __launch_bounds__(LP_THREADS, LP_CTAS) logprobs_kernel(LogprobAr
           at[q] = from.x + (j - entry * vecs) * LP_THREADS;
           if (at[q] < from.y) v[q] = __ldg(row.vec(at[q]));
         }
+        uint32_t hits = 0;
 #pragma unroll
         for (uint32_t q = 0; q < 4; q++) {
-          const float high = Vec<T>::high(v[q]);
-          if (!(high >= reach) || high == -INFINITY) continue;
-          const uint32_t first = row.head + at[q] * E;
-#pragma unroll 1
-          for (uint32_t e = 0; e < E; e++) offer(to_f32(row.x[first + e]), first + e, equal_too);
+          float x[E];
+          Vec<T>::unpack(v[q], x);
+#pragma unroll
+          for (int e = 0; e < E; e++) hits |= (uint32_t)(x[e] > reach || (x[e] == reach && equal_too)) << (q * E + e);
+        }
+        for (; hits; hits &= hits - 1) {
+          const uint32_t bit = __ffs(hits) - 1, q = bit / E, i = row.head + (q == 0 ? at[0] : q == 1 ? at[1] : q == 2 ? at[2] : at[3]) * E + bit % E;
+          offer(to_f32(row.x[i]), i, equal_too);
         }
       }
     }
