@@ -17,8 +17,10 @@
 // the shares' order: the same bits every time. Rows that fill the SMs stay whole (1500 of 50257 in f16, with 20 alternatives:
 // 43 us whole, 52 in two shares, 58 in three: a share's end, its reductions and barriers, costs more than evenness gives).
 //
-// Measured, with target, entropy, rank and alternatives: 1 row of 32000 (f32) 7.8 us, launch, two dependent reads and the
-// join; 64 of 151936 (f32) 19.5 us, 2.0 TB/s; 1500 of 50257 (f16) 43 us, 3.5 TB/s, 54 % of a copy's rate.
+// Measured, with target, entropy, rank and alternatives: 1 row of 32000 (f32) 6.3 us, a chain of dependent reads, the join and
+// the alternatives; 64 of 151936 (f32) 16.1 us, 2.4 TB/s, 9 of them the sweep and the rest the same chain; 1500 of 50257 (f16)
+// 42.8 us, 3.5 TB/s, 54 % of a copy's rate (the SMs' schedulers issue 60 % of the time, 20 warps each. Half the vectors in
+// flight and up to 11 CTAs on an SM: 47 to 51 us; 8 CTAs, with registers spilled: 41.6, and 18.3 for the 64 rows).
 #include <type_traits>
 
 #include "paged.cuh"

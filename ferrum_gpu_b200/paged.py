@@ -20,10 +20,13 @@ from .device import CudaError, Device
 
 _KINDS: dict = {}  # torch's element types -> FC_*, and ..
 _TYPES: dict = {}  # .. the other types by name: filled when the first tensor comes by (the package loads without torch)
+_INT32 = None      # torch.int32, then
 
 
 def _learn():
+    global _INT32
     import torch
+    _INT32 = torch.int32
     _KINDS.update({torch.float32: _ffi.FC_F32, torch.float16: _ffi.FC_F16, torch.bfloat16: _ffi.FC_BF16})
     _TYPES.update({"int32": torch.int32, "int64": torch.int64, "float32": torch.float32})
 
@@ -58,10 +61,10 @@ def _ints(dev: Device, t, name: str, n: int = 0):
     """The address of a contiguous int32 tensor of at least `n` entries on `dev`; None: NULL."""
     if t is None:
         return None
-    at, entries, where = _flat(t, name)
-    if where != dev.ordinal or entries < n:
+    if t.dtype is not _INT32 or t.get_device() != dev.ordinal or not t.is_contiguous() or (n and t.numel() < n):
+        _, entries, where = _flat(t, name)  # (the first tensor of all, or a fault: said there or here)
         _at(dev, name, n, entries, where)
-    return at
+    return t.data_ptr()
 
 
 def _at(dev: Device, name: str, n: int, entries: int, where: int):
