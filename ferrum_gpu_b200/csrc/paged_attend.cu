@@ -703,7 +703,7 @@ __global__ void __launch_bounds__(THREADS, Shape<C, HDP>::CTAS)
   // ---- the segments whose last part this CTA has written, joined by all four warps ----
   if (!wait_phase(&all_done, 0)) {
     if (lane == 0) atomicExch(a.err_flag, 6);
-    return; // (each warp by itself: without the verdict none of them may go on, and none waits for another)
+    return; // (each warp by itself: without it none of them knows what to join, and none waits for another)
   }
   for (uint32_t n = 0; n < sm_n_late; n++) {
     // Thread (part k of 16, head) weighs its parts; every thread adds up its channels, the first parts' values in flight
